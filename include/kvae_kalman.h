@@ -29,7 +29,10 @@ extern "C" {
 
 #define KVAE_ABI_VERSION 1
 
-enum { KVAE_F32 = 0, KVAE_F64 = 1 };
+enum {
+    KVAE_F32 = 0, KVAE_F64 = 1,
+    KVAE_BF16 = 2, KVAE_F16 = 3   /* sequence-network entry points and optimiser only */
+};
 
 enum {
     KVAE_OK = 0,
@@ -683,6 +686,92 @@ int kvae_weighted_terms(long n, int dtype, const void *terms, void *scratch, dou
  * ordering against dependent kernels is unreliable on ROCm 7.0.              */
 int kvae_graph_count_memset_nodes(void *hip_graph);
 int kvae_graph_count_kernel_nodes(void *hip_graph);
+
+/* ------------------------------------------------------------------------ */
+/* Gated linear recurrence, the sequence operator of the "gated" dynamics-parameter network (no
+ * counterpart in the reference, whose recurrent network is torch.nn.LSTM,
+ * kvae/dynamics_parameter_network.py:18-58).  Element-wise over (B,H), with u = [x | forget | o]
+ * along the last axis (gated != 0) or [x | forget]:
+ *   f_t = sigmoid(forget_t), c_t = f_t c_{t-1} + (1 - f_t) x_t, y_t = c_t o_t sigmoid(o_t) or c_t.
+ * Where mask is 0 the step is skipped: c_t = c_{t-1}, y_t = 0 and no gradient, whatever u holds
+ * there.  c_{-1} = h0, or 0 when that is NULL.
+ * dtype: KVAE_F32, KVAE_BF16 or KVAE_F16 for u, y, dy, du; the state is float throughout.
+ * u and dy have any strides over time and batch and stride 1 over the last axis; their address
+ * needs the element's alignment only.  y (T,B,H), du (T,B,3H or 2H), h0, last, dlast, dh0 (B,H)
+ * are contiguous and must not overlap the inputs.
+ * forward: writes y, last = c_{T-1} (or NULL) and, for a later backward call, states
+ *   (ceil(T / KVAE_SCAN_CHUNK), B, H): c before every KVAE_SCAN_CHUNK-th step (or NULL).
+ * backward: reads u, mask, states, dy and dlast (or NULL); writes du and dh0 (or NULL).
+ * Both need kvae_gated_scan_workspace_bytes() bytes (0 unless the time axis is split).       */
+#define KVAE_SCAN_CHUNK 16
+typedef struct {
+    int64_t T, B, H;
+    int32_t dtype;
+    int32_t gated;
+    const void *u;
+    int64_t u_stride_t, u_stride_b;         /* elements */
+    const void *mask;                       /* (T,B) bytes, or NULL = every step counts */
+    int64_t mask_stride_t, mask_stride_b;
+    const void *h0;
+    void *y, *last, *states;
+    const void *dy;
+    int64_t dy_stride_t, dy_stride_b;
+    const void *dlast;
+    void *du, *dh0;
+} kvae_gated_scan;
+
+size_t kvae_gated_scan_workspace_bytes(int64_t T, int64_t B, int64_t H, int dtype);
+int kvae_gated_scan_forward(const kvae_gated_scan *d, void *workspace, size_t workspace_bytes,
+                            void *stream);
+int kvae_gated_scan_backward(const kvae_gated_scan *d, void *workspace, size_t workspace_bytes,
+                             void *stream);
+/* One step: u (B,3H or 2H) with row stride u_stride_b, mask (B) bytes or NULL, state (B,H) float
+ * read and written, y (B,H).                                                                */
+int kvae_gated_scan_step(int64_t B, int64_t H, int dtype, int gated, const void *u,
+                         int64_t u_stride_b, const void *mask, int64_t mask_stride_b, void *state,
+                         void *y, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Root-mean-square norm of rows with the residual's addition, around the recurrence of the "gated"
+ * dynamics-parameter network (no counterpart in the reference):
+ *   r = x + residual (or x), y = r (mean r^2 + eps)^(-1/2) weight.
+ * dtype: KVAE_F32, KVAE_BF16 or KVAE_F16 for x, residual, y, sum, dy, dsum and dx; weight and
+ * dweight have weight_dtype, which is KVAE_F32 or dtype; r and all sums are float.  Inputs have a row
+ * stride (elements) and need the element's alignment only; outputs are contiguous.  D up to
+ * KVAE_NORM_MAX_WIDTH.
+ * forward: writes y and, where not NULL, sum (rows,D) = r rounded to dtype and rstd (rows) float =
+ *   the inverse root (the backward call needs it).
+ * quantized: y (rows,D) in e4m3 bytes and scale (rows) float with y = q scale:
+ *   scale = max(max |y| / 448, 2^-126), to the nearest; a NaN stays one and does not enter the scale.
+ * backward: r is formed again from x and residual (or pass the stored sum as x and residual = NULL);
+ *   writes dx = the gradient w.r.t. x and w.r.t. residual alike, with dsum (or NULL), the gradient
+ *   that reaches sum, added; and dweight.  partial: kvae_rms_norm_backward_parts(rows) x D floats.
+ * kvae_quantize_rows: the same e4m3 form of the rows of x as they are.                        */
+#define KVAE_NORM_MAX_WIDTH 16384
+typedef struct {
+    int64_t rows, D;
+    int32_t dtype, weight_dtype;
+    const void *x;
+    int64_t x_stride;
+    const void *residual;
+    int64_t residual_stride;
+    const void *weight;
+    float eps;
+    int32_t _pad;
+    void *y, *scale, *sum, *rstd;           /* scale: quantized only */
+    const void *dy;
+    int64_t dy_stride;
+    const void *dsum;
+    int64_t dsum_stride;
+    void *dx, *partial, *dweight;
+} kvae_rms_norm;
+
+int64_t kvae_rms_norm_backward_parts(int64_t rows);
+int kvae_rms_norm_forward(const kvae_rms_norm *d, void *stream);
+int kvae_rms_norm_quantized(const kvae_rms_norm *d, void *stream);
+int kvae_rms_norm_backward(const kvae_rms_norm *d, void *stream);
+int kvae_quantize_rows(int64_t rows, int64_t D, int dtype, const void *x, int64_t x_stride, void *q,
+                       void *scale, void *stream);
 
 /* ------------------------------------------------------------------------ */
 enum {

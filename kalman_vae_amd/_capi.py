@@ -13,7 +13,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # KVAE_LIB_PATH: another build of the same library (kernel experiments)
 LIB_PATH = os.environ.get("KVAE_LIB_PATH") or os.path.join(_HERE, "csrc", "libkvae_kalman.so")
 
-KVAE_F32, KVAE_F64 = 0, 1
+KVAE_F32, KVAE_F64, KVAE_BF16, KVAE_F16 = 0, 1, 2, 3
+SCAN_CHUNK = 16
 OP_FILTER_BWD, OP_SMOOTH_BWD, OP_ELBO_BWD, OP_LOSS_FWD, OP_LOSS_BWD = 1, 2, 3, 4, 5
 OP_LOSS_VALUE_AND_GRAD = 6
 
@@ -78,6 +79,18 @@ Rollout = _ptr_struct("Rollout", [
     ("hidden", C.c_int32), ("phase", C.c_int32), ("sample", C.c_int32), ("_pad", C.c_int32),
     "as_new", "means", "covs", "mean_pred_new", "cov_pred_new", "mat_As_new", "mat_Cs_new",
     "status"])
+_i64 = C.c_int64
+GatedScan = _ptr_struct("GatedScan", [
+    ("T", _i64), ("B", _i64), ("H", _i64), ("dtype", C.c_int32), ("gated", C.c_int32),
+    "u", ("u_stride_t", _i64), ("u_stride_b", _i64),
+    "mask", ("mask_stride_t", _i64), ("mask_stride_b", _i64), "h0", "y", "last", "states",
+    "dy", ("dy_stride_t", _i64), ("dy_stride_b", _i64), "dlast", "du", "dh0"])
+RmsNorm = _ptr_struct("RmsNorm", [
+    ("rows", _i64), ("D", _i64), ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+    "x", ("x_stride", _i64), "residual", ("residual_stride", _i64), "weight",
+    ("eps", C.c_float), ("_pad", C.c_int32), "y", "scale", "sum", "rstd",
+    "dy", ("dy_stride", _i64), "dsum", ("dsum_stride", _i64), "dx", "partial", "dweight"])
+NORM_MAX_WIDTH = 16384
 ROLLOUT_ALL, ROLLOUT_EMIT, ROLLOUT_ADVANCE = 0, 1, 2
 
 EXPORTS = (
@@ -105,6 +118,10 @@ EXPORTS = (
     "kvae_graph_count_memset_nodes", "kvae_graph_count_kernel_nodes",
     "kvae_column_sum", "kvae_column_sum_many", "kvae_vector_sum", "kvae_vector_sum_scratch_elems",
     "kvae_weighted_terms", "kvae_weighted_terms_scratch_elems",
+    "kvae_gated_scan_workspace_bytes", "kvae_gated_scan_forward", "kvae_gated_scan_backward",
+    "kvae_gated_scan_step",
+    "kvae_rms_norm_backward_parts", "kvae_rms_norm_forward", "kvae_rms_norm_quantized",
+    "kvae_rms_norm_backward", "kvae_quantize_rows",
 )
 
 
@@ -115,6 +132,11 @@ def ptr(t):
     if not t.is_contiguous():
         raise ValueError("tensor passed to the Kalman kernels must be contiguous")
     return t.data_ptr()
+
+
+def ptr_strided(t):
+    """Device address of a tensor whose strides go with it; None -> NULL."""
+    return None if t is None else t.data_ptr()
 
 
 def fill(struct, **tensors):
@@ -132,6 +154,16 @@ def dtype_code(dtype):
     if dtype == torch.float64:
         return KVAE_F64
     raise TypeError(f"Kalman kernels support float32 and float64, got {dtype}")
+
+
+SEQUENCE_DTYPES = {torch.float32: KVAE_F32, torch.bfloat16: KVAE_BF16, torch.float16: KVAE_F16}
+
+
+def sequence_dtype_code(dtype):
+    """Element type of the sequence-network operators and the optimiser."""
+    if dtype not in SEQUENCE_DTYPES:
+        raise TypeError(f"float32, bfloat16 or float16 expected, got {dtype}")
+    return SEQUENCE_DTYPES[dtype]
 
 
 _lib = None
@@ -282,6 +314,21 @@ def load():
     lib.kvae_vector_sum.restype = C.c_int
     lib.kvae_vector_sum_scratch_elems.argtypes = [C.c_int, C.c_long]
     lib.kvae_vector_sum_scratch_elems.restype = C.c_long
+    lib.kvae_gated_scan_workspace_bytes.argtypes = [_i64] * 3 + [C.c_int]
+    lib.kvae_gated_scan_workspace_bytes.restype = C.c_size_t
+    for name in ("kvae_gated_scan_forward", "kvae_gated_scan_backward"):
+        getattr(lib, name).argtypes = [C.POINTER(GatedScan), _vp, C.c_size_t, _vp]
+        getattr(lib, name).restype = C.c_int
+    lib.kvae_gated_scan_step.argtypes = [_i64, _i64, C.c_int, C.c_int, _vp, _i64, _vp, _i64, _vp, _vp,
+                                         _vp]
+    lib.kvae_gated_scan_step.restype = C.c_int
+    lib.kvae_rms_norm_backward_parts.argtypes = [_i64]
+    lib.kvae_rms_norm_backward_parts.restype = _i64
+    for name in ("kvae_rms_norm_forward", "kvae_rms_norm_quantized", "kvae_rms_norm_backward"):
+        getattr(lib, name).argtypes = [C.POINTER(RmsNorm), _vp]
+        getattr(lib, name).restype = C.c_int
+    lib.kvae_quantize_rows.argtypes = [_i64, _i64, C.c_int, _vp, _i64, _vp, _vp, _vp]
+    lib.kvae_quantize_rows.restype = C.c_int
     _lib = lib
     return lib
 

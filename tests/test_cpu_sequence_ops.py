@@ -1,0 +1,114 @@
+"""Refusals of the sequence-network operators and of their C entry points: every one comes from the
+host, before anything is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+import kalman_vae_amd as kv
+from kalman_vae_amd import _capi as capi
+
+
+def test_no_cpu_path():
+    u, w = torch.zeros(3, 2, 12), torch.ones(12)
+    for call in (lambda: kv.gated_scan(u), lambda: kv.gated_scan_step(u[0], torch.zeros(2, 4)),
+                 lambda: kv.rms_norm(u, w), lambda: kv.rms_norm_quantized(u, w), lambda: kv.quantize_rows(u)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+def as_if_on_gpu(monkeypatch):
+    """The argument checks run on any tensor; what follows them is not reached in these tests."""
+    from kalman_vae_amd import sequence_ops
+    monkeypatch.setattr(sequence_ops, "_device_of", lambda *t: torch.device("cpu"))
+
+
+@pytest.mark.parametrize("call,error,match", [
+    (lambda: kv.gated_scan(torch.zeros(3, 12)), ValueError, "shape"),
+    (lambda: kv.gated_scan(torch.zeros(3, 2, 13)), ValueError, "3 equal parts"),
+    (lambda: kv.gated_scan(torch.zeros(3, 2, 13), output_gate=False), ValueError, "2 equal parts"),
+    (lambda: kv.gated_scan(torch.zeros(3, 2, 12).double()), TypeError, "float64"),
+    (lambda: kv.gated_scan(torch.zeros(3, 2, 12), torch.zeros(2, 5)), ValueError, "h0 must have shape"),
+    (lambda: kv.gated_scan(torch.zeros(3, 2, 12), torch.zeros(2, 4).half()), TypeError, "float32"),
+    (lambda: kv.gated_scan(torch.zeros(3, 2, 12), mask=torch.zeros(2, 3)), ValueError, "mask must have"),
+    (lambda: kv.gated_scan_step(torch.zeros(3, 2, 12), torch.zeros(2, 4)), ValueError, "shape"),
+    (lambda: kv.gated_scan_step(torch.zeros(2, 12), torch.zeros(2, 8)[:, ::2]), ValueError, "contiguous"),
+    (lambda: kv.gated_scan_step(torch.zeros(2, 12), torch.zeros(2, 4), mask=torch.zeros(3)), ValueError, "mask"),
+    (lambda: kv.gated_scan_step(torch.zeros(2, 12, requires_grad=True), torch.zeros(2, 4)), RuntimeError, "no gradient"),
+    (lambda: kv.rms_norm(torch.zeros(3, 4), torch.ones(5)), ValueError, "weight must have shape"),
+    (lambda: kv.rms_norm(torch.zeros(3, 4), torch.ones(4).half()), TypeError, "weight must be"),
+    (lambda: kv.rms_norm(torch.zeros(()), torch.ones(4)), ValueError, "one axis"),
+    (lambda: kv.rms_norm(torch.zeros(3, 4).long(), torch.ones(4)), TypeError, "int64"),
+    (lambda: kv.rms_norm(torch.zeros(3, 4), torch.ones(4), residual=torch.zeros(4)), ValueError, "residual"),
+    (lambda: kv.rms_norm(torch.zeros(3, 4), torch.ones(4), residual=torch.zeros(3, 4).half()), TypeError, "residual"),
+    (lambda: kv.rms_norm(torch.zeros(1, 16385), torch.ones(16385)), NotImplementedError, "16384"),
+    (lambda: kv.rms_norm_quantized(torch.zeros(3, 4), torch.ones(4, requires_grad=True)), RuntimeError, "no gradient"),
+    (lambda: kv.quantize_rows(torch.zeros(3, 4, requires_grad=True)), RuntimeError, "no gradient"),
+    (lambda: kv.quantize_rows(torch.zeros(1, 16385)), NotImplementedError, "16384"),
+])
+def test_refusals(monkeypatch, call, error, match):
+    as_if_on_gpu(monkeypatch)
+    with pytest.raises(error, match=match):
+        call()
+
+
+def test_c_entry_points_refuse_before_launching():
+    lib = capi.load()
+    one = 4096                                   # an address that is never followed
+    d = capi.GatedScan(T=4, B=2, H=8, dtype=capi.KVAE_F32, gated=1)
+    assert lib.kvae_gated_scan_forward(C.byref(d), None, 0, None) == -1            # no u
+    d.u = one
+    assert lib.kvae_gated_scan_forward(C.byref(d), None, 0, None) == -1            # no y
+    d.y, d.dtype = one, capi.KVAE_F64
+    assert lib.kvae_gated_scan_forward(C.byref(d), None, 0, None) == -2
+    d.dtype, d.T = capi.KVAE_F32, 0
+    assert lib.kvae_gated_scan_forward(C.byref(d), None, 0, None) == -1
+    d.T = 1 << 20                                # cut into segments: needs a workspace
+    need = lib.kvae_gated_scan_workspace_bytes(d.T, d.B, d.H, d.dtype)
+    assert need > 0 and lib.kvae_gated_scan_forward(C.byref(d), one, need - 1, None) == -3
+    assert lib.kvae_gated_scan_backward(C.byref(d), one, need, None) == -1         # no states, dy, du
+    d.T, d.B, d.H = 1, 1 << 30, 1 << 20
+    assert lib.kvae_gated_scan_forward(C.byref(d), None, 0, None) == -5
+    assert lib.kvae_gated_scan_forward(None, None, 0, None) == -1
+    assert lib.kvae_gated_scan_step(2, 8, 9, 1, one, 24, None, 0, one, one, None) == -2
+    assert lib.kvae_gated_scan_step(2, 8, 0, 1, None, 24, None, 0, one, one, None) == -1
+    n = capi.RmsNorm(rows=2, D=8, dtype=capi.KVAE_F32, weight_dtype=capi.KVAE_F32, x=one, weight=one)
+    assert lib.kvae_rms_norm_forward(C.byref(n), None) == -1                       # no y
+    n.y = one
+    assert lib.kvae_rms_norm_quantized(C.byref(n), None) == -1                     # no scale
+    assert lib.kvae_rms_norm_backward(C.byref(n), None) == -1
+    n.weight_dtype = capi.KVAE_BF16
+    assert lib.kvae_rms_norm_forward(C.byref(n), None) == -2
+    n.weight_dtype, n.D = capi.KVAE_F32, 16385
+    assert lib.kvae_rms_norm_forward(C.byref(n), None) == -2
+    n.D, n.rows = 8, 1 << 32
+    assert lib.kvae_rms_norm_forward(C.byref(n), None) == -5
+    assert lib.kvae_quantize_rows(2, 8, 1, one, 8, one, one, None) == -2
+    assert lib.kvae_quantize_rows(2, 8, 0, one, 8, None, one, None) == -1
+
+
+def test_segments_of_the_time_axis():
+    """The workspace says how the time axis is cut: not at all for short sequences or many channels,
+    and never into segments of fewer than two chunks."""
+    lib = capi.load()
+    size = lambda T, B, H, d=0: lib.kvae_gated_scan_workspace_bytes(T, B, H, d)  # noqa: E731
+    assert size(1, 1, 1) == size(63, 1, 1) == size(1000, 4096, 128) == 0
+    for T in (64, 1000, 32768, 1 << 22):
+        for B, H, d in ((1, 1, 0), (1, 520, 3), (3, 65, 2)):
+            segs = size(T, B, H, d) / (12 * B * H)
+            assert segs == int(segs) and segs <= T / 32, (T, B, H, d)
+
+
+def test_ctypes_structs_match_header(tmp_path):
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = {"kvae_gated_scan": (capi.GatedScan, "dh0"), "kvae_rms_norm": (capi.RmsNorm, "dweight")}
+    src = '#include <stdio.h>\n#include "kvae_kalman.h"\nint main(void){\n'
+    for n, (_, last) in names.items():
+        src += f'printf("%zu %zu\\n", sizeof({n}), offsetof({n}, {last}));\n'
+    (tmp_path / "s.c").write_text(src + "return 0;}\n")
+    subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")])
+    lines = subprocess.check_output([str(tmp_path / "s")], text=True).splitlines()
+    for line, (cls, last) in zip(lines, names.values()):
+        assert line == f"{C.sizeof(cls)} {getattr(cls, last).offset}"
