@@ -774,6 +774,42 @@ int kvae_quantize_rows(int64_t rows, int64_t D, int dtype, const void *x, int64_
                        void *scale, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* AdamW (decoupled weight decay) over up to KVAE_ADAMW_MAX_TENSORS tensors in one launch: the
+ * optimiser step of a training loop (examples/train.py:126-131 steps torch.optim.Adam).
+ *   m = b1 m + (1-b1) g, v = b2 v + (1-b2) g^2,
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * dtype: KVAE_F32, KVAE_BF16 or KVAE_F16 of param and grad.  master: a float copy of a 16-bit
+ * parameter that is updated in its place (param receives it rounded), in all tensors of a call or
+ * in none.  All tensors contiguous, at any element-aligned address.
+ * state_bits 32: exp_avg, exp_avg_sq hold m and v in float.  state_bits 8: e4m3 bytes of m and of
+ * sqrt(v), with a float scale per KVAE_ADAMW_BLOCK elements (the last block may be short); rounded
+ * up or down by a hash of (seed, t, first_block * KVAE_ADAMW_BLOCK + element), first_block counting
+ * the blocks of the tensors of earlier calls of the same step, so that no two share their bits.  A
+ * positive sqrt(v) never gets the code 0.
+ * t = step >= 1, or *step_device (int64) when that is not NULL: then the launch may be captured and
+ * replayed; lr_device (float, or NULL) likewise replaces lr.                                 */
+#define KVAE_ADAMW_BLOCK 256
+#define KVAE_ADAMW_MAX_TENSORS 48
+typedef struct {
+    int64_t numel;
+    void *param;
+    const void *grad;
+    void *exp_avg, *exp_avg_sq;
+    void *exp_avg_scale, *exp_avg_sq_scale;
+    void *master;
+} kvae_adamw_tensor;
+typedef struct {
+    const kvae_adamw_tensor *tensors;       /* host array, read before the call returns */
+    int32_t count, dtype, state_bits;
+    uint32_t seed;
+    int64_t step, first_block;
+    double lr, beta1, beta2, eps, weight_decay;
+    const void *step_device, *lr_device;
+} kvae_adamw;
+
+int kvae_adamw_step(const kvae_adamw *d, void *stream);
+
+/* ------------------------------------------------------------------------ */
 enum {
     KVAE_OP_FILTER_BWD = 1, KVAE_OP_SMOOTH_BWD = 2, KVAE_OP_ELBO_BWD = 3,
     KVAE_OP_LOSS_FWD = 4, KVAE_OP_LOSS_BWD = 5, KVAE_OP_LOSS_VALUE_AND_GRAD = 6

@@ -91,6 +91,11 @@ RmsNorm = _ptr_struct("RmsNorm", [
     ("eps", C.c_float), ("_pad", C.c_int32), "y", "scale", "sum", "rstd",
     "dy", ("dy_stride", _i64), "dsum", ("dsum_stride", _i64), "dx", "partial", "dweight"])
 NORM_MAX_WIDTH = 16384
+AdamW = _ptr_struct("AdamW", [
+    "tensors", ("count", C.c_int32), ("dtype", C.c_int32), ("state_bits", C.c_int32),
+    ("seed", C.c_uint32), ("step", _i64), ("first_block", _i64), ("lr", C.c_double),
+    ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+    "step_device", "lr_device"])
 ROLLOUT_ALL, ROLLOUT_EMIT, ROLLOUT_ADVANCE = 0, 1, 2
 
 EXPORTS = (
@@ -121,7 +126,7 @@ EXPORTS = (
     "kvae_gated_scan_workspace_bytes", "kvae_gated_scan_forward", "kvae_gated_scan_backward",
     "kvae_gated_scan_step",
     "kvae_rms_norm_backward_parts", "kvae_rms_norm_forward", "kvae_rms_norm_quantized",
-    "kvae_rms_norm_backward", "kvae_quantize_rows",
+    "kvae_rms_norm_backward", "kvae_quantize_rows", "kvae_adamw_step",
 )
 
 
@@ -329,6 +334,8 @@ def load():
         getattr(lib, name).restype = C.c_int
     lib.kvae_quantize_rows.argtypes = [_i64, _i64, C.c_int, _vp, _i64, _vp, _vp, _vp]
     lib.kvae_quantize_rows.restype = C.c_int
+    lib.kvae_adamw_step.argtypes = [C.POINTER(AdamW), _vp]
+    lib.kvae_adamw_step.restype = C.c_int
     _lib = lib
     return lib
 

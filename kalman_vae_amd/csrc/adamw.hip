@@ -1,0 +1,300 @@
+// AdamW step over many tensors in one launch, on gfx950, with the states in float or in 8 bits:
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// A stream over memory: parameter, gradient and both states are read once and written once (float:
+// 28 bytes an element; 8-bit states: 16 bytes).  The tensors' addresses travel with the launch, so
+// a model of some forty small tensors costs one launch; a workgroup finds its tensor by bisection.
+//
+// 8-bit states.  Blocks of 256 elements hold m and sqrt(v) as e4m3 values times one scale per
+// block (max / 448).  sqrt(v) and not v: e4m3 spans 2^18 between its largest and its smallest
+// positive value, so v spans 2^36 within a block.  Two rules keep training sound:
+// - Rounding is stochastic.  v moves by a thousandth of itself a step (b2 = 0.999) and the code's
+//   step is a sixteenth: to the nearest it would never move.  The random bits are a hash of
+//   (seed, step, index), so a run can be repeated bit for bit.
+// - The code of a positive sqrt(v) is never zero: the update divides by it, and a zero under an m
+//   that was rounded up would make a step of a thousand times lr.
+// The arithmetic of the states is written without contraction into fused multiply-adds and with
+// correctly rounded roots and reciprocals: codes come out the same as from the formulas
+// above evaluated one operation at a time.
+#include "narrow_types.h"
+
+namespace kvae {
+
+constexpr int ADAM_THREADS = 256;
+constexpr int PER_LANE = 16;                         // elements: 16 lanes hold a block of 256
+constexpr int ADAM_CHUNK = ADAM_THREADS * PER_LANE;  // elements of a workgroup
+constexpr int QUANT_BLOCK = KVAE_ADAMW_BLOCK;
+constexpr int TABLE = KVAE_ADAMW_MAX_TENSORS;
+static_assert(QUANT_BLOCK == 16 * PER_LANE, "a block is one row of 16 lanes");
+
+struct AdamArgs {
+    kvae_adamw_tensor t[TABLE];
+    int first_chunk[TABLE + 1];                      // workgroup -> tensor
+    unsigned first_block[TABLE];                     // blocks of 256 of the tensors before (hash index)
+    int count;
+    float lr, beta1, beta2, eps, decay;              // decay: lr * weight_decay
+    float one_minus_beta1, one_minus_beta2;
+    float rate, root_fix;                            // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+    unsigned key;                                    // seed + t * 0x9E3779B9
+    double dbeta1, dbeta2, dlr, ddecay;              // for a step count that lives on the device
+    const int64_t* step;
+    const float* lr_device;
+    unsigned seed;
+};
+
+template <int CTRL>
+__device__ __forceinline__ float row_exchange(float x) {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float max16(float v) {
+    v = fmaxf(v, row_exchange<0xB1>(v));
+    v = fmaxf(v, row_exchange<0x4E>(v));
+    v = fmaxf(v, row_exchange<0x141>(v));
+    return fmaxf(v, row_exchange<0x140>(v));
+}
+
+constexpr float E4M3_MAX = 448.f;
+constexpr float SMALLEST_SCALE = 1.17549435e-38f;    // smallest normal: its reciprocal is finite
+
+// Two rounds of multiply and shift (C. Wellons' 32-bit mix) over a multiplicative start.
+__device__ __forceinline__ unsigned random_bits(unsigned index, unsigned key) {
+    unsigned h = index * 0x9E3779B1u + key;
+    h = (h ^ (h >> 16)) * 0x7FEB352Du;
+    h = (h ^ (h >> 15)) * 0x846CA68Bu;
+    return h ^ (h >> 16);
+}
+
+// t >= 0 to an e4m3 value, up or down by 16 random bits; POSITIVE: never to zero unless t is.
+template <bool POSITIVE>
+__device__ __forceinline__ float round_e4m3(float t, unsigned random16) {
+    t = t > E4M3_MAX ? E4M3_MAX : t;                 // (a NaN stays)
+    const unsigned bits = __builtin_bit_cast(unsigned, t) + (random16 << 4) + 8u;
+    float normal = __builtin_bit_cast(float, bits & ~0xFFFFFu);
+    normal = normal > E4M3_MAX ? E4M3_MAX : normal;
+    float small = floorf(__fadd_rn(t * 512.f, ((float)random16 + 0.5f) * (1.f / 65536.f)));
+    if constexpr (POSITIVE) small = t > 0.f ? fmaxf(small, 1.f) : 0.f;
+    return t < 0.015625f ? small * (1.f / 512.f) : (t == t ? normal : t);
+}
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
+}
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, int n, float (&x)[PER_LANE]) {
+    constexpr int V = 16 / sizeof(T);
+    if (n >= PER_LANE) {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; i += V) {
+            const Pack<T, V> q = load_pack<T, V>(p + i);
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[i + v] = widen(q.v[v]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i) x[i] = i < n ? widen(p[i]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, int n, const float (&x)[PER_LANE]) {
+    constexpr int V = 16 / sizeof(T);
+    if (n >= PER_LANE) {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; i += V) {
+            Pack<T, V> q;
+#pragma unroll
+            for (int v = 0; v < V; ++v) q.v[v] = narrow<T>(x[i + v]);
+            store_pack<T, V>(p + i, q);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i)
+            if (i < n) p[i] = narrow<T>(x[i]);
+    }
+}
+// sixteen e4m3 bytes
+__device__ __forceinline__ void load_codes(const uint8_t* p, int n, float scale, float (&x)[PER_LANE]) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (n >= PER_LANE) {
+        struct __attribute__((packed)) Any { uint32_t w[4]; };
+        const Any a = *reinterpret_cast<const Any*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = a.w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i)
+            if (i < n) w[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(w[i], 0) * scale;
+        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(w[i], 1) * scale;
+        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(w[i], 2) * scale;
+        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(w[i], 3) * scale;
+    }
+}
+// Codes and scale of a block of 256 over a row of 16 lanes.  SHIFT: which half of the hash decides.
+template <bool POSITIVE, int SHIFT>
+__device__ __forceinline__ void store_codes(uint8_t* p, float* scale_at, bool first, int n,
+                                            const float (&x)[PER_LANE], unsigned index, unsigned key) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) big = fmaxf(big, fabsf(x[i]));
+    big = max16(big);
+    const float scale = fmaxf(big * (1.f / E4M3_MAX), SMALLEST_SCALE);
+    const float inverse = 1.f / scale;
+    if (first) *scale_at = scale;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float q[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float t = x[4 * i + k] * inverse;
+            const unsigned r = random_bits(index + 4 * i + k, key);
+            q[k] = copysignf(round_e4m3<POSITIVE>(fabsf(t), SHIFT ? r >> 16 : r & 0xFFFFu), t);
+        }
+        w[i] = pack_e4m3(q[0], q[1], q[2], q[3]);
+    }
+    if (n >= PER_LANE) {
+        struct __attribute__((packed)) Any { uint32_t w[4]; };
+        Any a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a.w[i] = w[i];
+        *reinterpret_cast<Any*>(p) = a;
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i)
+            if (i < n) p[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+}
+
+template <typename T, bool EIGHT, bool MASTER>
+__global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const AdamArgs g) {
+#pragma clang fp contract(off)
+    __shared__ float fixes[2];
+    float lr = g.lr, decay = g.decay, rate = g.rate, root_fix = g.root_fix;
+    unsigned key = g.key;
+    if (g.step) {                                    // captured: step count and rate live on the device
+        if (threadIdx.x == 0) {
+            const double t = (double)*g.step;
+            const double rate1 = g.lr_device ? (double)*g.lr_device : g.dlr;
+            fixes[0] = (float)(rate1 / -expm1(t * log(g.dbeta1)));
+            fixes[1] = (float)(1.0 / sqrt(-expm1(t * log(g.dbeta2))));
+        }
+        __syncthreads();
+        rate = fixes[0];
+        root_fix = fixes[1];
+        lr = g.lr_device ? *g.lr_device : lr;
+        decay = (float)((g.lr_device ? (double)*g.lr_device : g.dlr) * g.ddecay);
+        key = g.seed + (unsigned)*g.step * 0x9E3779B9u;
+    }
+    int low = 0, high = g.count;                     // first_chunk[low] <= blockIdx.x < first_chunk[high]
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (g.first_chunk[mid] <= (int)blockIdx.x) low = mid; else high = mid;
+    }
+    const kvae_adamw_tensor t = g.t[low];
+    const long at = (long)(blockIdx.x - g.first_chunk[low]) * ADAM_CHUNK + (long)threadIdx.x * PER_LANE;
+    const long left = t.numel - at;
+    const int n = left >= PER_LANE ? PER_LANE : (left > 0 ? (int)left : 0);
+    const long block = at / QUANT_BLOCK;
+    // a row of 16 lanes (one block) leaves together, so that max16 finds all its lanes
+    if (block * QUANT_BLOCK >= t.numel) return;
+    float p[PER_LANE], grad[PER_LANE], m[PER_LANE], v[PER_LANE];
+    if constexpr (MASTER) {
+        load16<float>(static_cast<const float*>(t.master) + at, n, p);
+    } else {
+        load16<T>(static_cast<const T*>(t.param) + at, n, p);
+    }
+    load16<T>(static_cast<const T*>(t.grad) + at, n, grad);
+    if constexpr (EIGHT) {
+        load_codes(static_cast<const uint8_t*>(t.exp_avg) + at, n,
+                   static_cast<const float*>(t.exp_avg_scale)[block], m);
+        load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at, n,
+                   static_cast<const float*>(t.exp_avg_sq_scale)[block], v);
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i) v[i] = v[i] * v[i];
+    } else {
+        load16<float>(static_cast<const float*>(t.exp_avg) + at, n, m);
+        load16<float>(static_cast<const float*>(t.exp_avg_sq) + at, n, v);
+    }
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) {
+        m[i] = m[i] * g.beta1 + grad[i] * g.one_minus_beta1;
+        v[i] = v[i] * g.beta2 + (grad[i] * grad[i]) * g.one_minus_beta2;
+        const float root = sqrtf(v[i]);
+        if constexpr (EIGHT) v[i] = root;            // from here on sqrt(v)
+        p[i] = p[i] * (1.f - decay) - rate * (m[i] / (root * root_fix + g.eps));
+    }
+    if constexpr (MASTER) store16<float>(static_cast<float*>(t.master) + at, n, p);
+    store16<T>(static_cast<T*>(t.param) + at, n, p);
+    if constexpr (EIGHT) {
+        const bool first = at == block * QUANT_BLOCK;
+        const unsigned index = g.first_block[low] * (unsigned)QUANT_BLOCK + (unsigned)at;
+        store_codes<false, 0>(static_cast<uint8_t*>(t.exp_avg) + at,
+                              static_cast<float*>(t.exp_avg_scale) + block, first, n, m, index, key);
+        store_codes<true, 1>(static_cast<uint8_t*>(t.exp_avg_sq) + at,
+                             static_cast<float*>(t.exp_avg_sq_scale) + block, first, n, v, index, key);
+    } else {
+        store16<float>(static_cast<float*>(t.exp_avg) + at, n, m);
+        store16<float>(static_cast<float*>(t.exp_avg_sq) + at, n, v);
+    }
+}
+
+}  // namespace kvae
+
+using namespace kvae;
+
+extern "C" int kvae_adamw_step(const kvae_adamw* d, void* stream) {
+    if (!d || d->count < 1 || d->count > TABLE || !d->tensors) return KVAE_E_BADARG;
+    if (d->state_bits != 32 && d->state_bits != 8) return KVAE_E_UNSUPPORTED;
+    if (d->dtype != KVAE_F32 && d->dtype != KVAE_BF16 && d->dtype != KVAE_F16) return KVAE_E_UNSUPPORTED;
+    if (!d->step_device && d->step < 1) return KVAE_E_BADARG;
+    static_assert(sizeof(AdamArgs) <= 4096, "arguments of a launch");
+    AdamArgs g{};
+    long chunks = 0, blocks = d->first_block;
+    const bool master = d->tensors[0].master != nullptr;
+    for (int i = 0; i < d->count; ++i) {
+        const kvae_adamw_tensor& t = d->tensors[i];
+        if (t.numel < 1 || !t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return KVAE_E_BADARG;
+        if (d->state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return KVAE_E_BADARG;
+        if ((t.master != nullptr) != master) return KVAE_E_BADARG;
+        g.t[i] = t;
+        g.first_chunk[i] = (int)chunks;
+        g.first_block[i] = (unsigned)blocks;
+        chunks += (t.numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
+        blocks += (t.numel + QUANT_BLOCK - 1) / QUANT_BLOCK;
+        if (chunks > 0x7fffffffL) return KVAE_E_TOOLARGE;
+    }
+    g.first_chunk[d->count] = (int)chunks;
+    g.count = d->count;
+    g.lr = (float)d->lr, g.beta1 = (float)d->beta1, g.beta2 = (float)d->beta2, g.eps = (float)d->eps;
+    g.one_minus_beta1 = (float)(1.0 - d->beta1), g.one_minus_beta2 = (float)(1.0 - d->beta2);
+    g.decay = (float)(d->lr * d->weight_decay);
+    g.dbeta1 = d->beta1, g.dbeta2 = d->beta2, g.dlr = d->lr, g.ddecay = d->weight_decay;
+    g.step = static_cast<const int64_t*>(d->step_device);
+    g.lr_device = static_cast<const float*>(d->lr_device);
+    g.seed = d->seed;
+    if (!g.step) {
+        g.rate = (float)(d->lr / (1.0 - pow(d->beta1, (double)d->step)));
+        g.root_fix = (float)(1.0 / sqrt(1.0 - pow(d->beta2, (double)d->step)));
+        g.key = d->seed + (unsigned)d->step * 0x9E3779B9u;
+    }
+    return for_element_type(d->dtype, [&](auto e) {
+        using T = decltype(e);
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        const auto go = [&](auto eight, auto with_master) {
+            adamw_kernel<T, decltype(eight)::value, decltype(with_master)::value>
+                <<<dim3((unsigned)chunks), ADAM_THREADS, 0, s>>>(g);
+        };
+        const auto with_bits = [&](auto with_master) {
+            d->state_bits == 8 ? go(std::true_type{}, with_master) : go(std::false_type{}, with_master);
+        };
+        master ? with_bits(std::true_type{}) : with_bits(std::false_type{});
+        return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
+    });
+}

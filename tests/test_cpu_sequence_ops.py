@@ -103,7 +103,8 @@ def test_ctypes_structs_match_header(tmp_path):
     import os
     import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    names = {"kvae_gated_scan": (capi.GatedScan, "dh0"), "kvae_rms_norm": (capi.RmsNorm, "dweight")}
+    names = {"kvae_gated_scan": (capi.GatedScan, "dh0"), "kvae_rms_norm": (capi.RmsNorm, "dweight"),
+             "kvae_adamw": (capi.AdamW, "lr_device")}
     src = '#include <stdio.h>\n#include "kvae_kalman.h"\nint main(void){\n'
     for n, (_, last) in names.items():
         src += f'printf("%zu %zu\\n", sizeof({n}), offsetof({n}, {last}));\n'
@@ -112,3 +113,56 @@ def test_ctypes_structs_match_header(tmp_path):
     lines = subprocess.check_output([str(tmp_path / "s")], text=True).splitlines()
     for line, (cls, last) in zip(lines, names.values()):
         assert line == f"{C.sizeof(cls)} {getattr(cls, last).offset}"
+
+
+def test_adamw_refusals(monkeypatch):
+    from kalman_vae_amd import AdamW, adamw_step
+    z = lambda n=4, d=torch.float32: torch.zeros(n, dtype=d)  # noqa: E731
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        adamw_step([z()], [z()], [z()], [z()], 1)
+    monkeypatch.setattr(capi, "require_gpu", lambda *t: None)
+    p = z()
+    codes, scale = z(4, torch.float8_e4m3fn), z(1)
+    for args, error, match in [
+            (([p], [z(5)], [z()], [z()], 1), ValueError, "elements"),
+            (([p], [z().double()], [z()], [z()], 1), TypeError, "float64"),
+            (([z().double()], [z()], [z()], [z()], 1), TypeError, "float64"),
+            (([p], [], [z()], [z()], 1), ValueError, "0 gradients for 1"),
+            (([p], [z()], [z().half()], [z()], 1), TypeError, "exp_avgs"),
+            (([p], [z(8)[::2]], [z()], [z()], 1), ValueError, "contiguous"),
+            (([p, p], [z(), z()], [z(), z()], [z(), z()], 1), ValueError, "twice"),
+            (([p], [z()], [z()], [z()], 0), ValueError, "counts from 1"),
+            (([p], [z()], [z()], [z()], torch.zeros(1)), ValueError, "int64"),
+            (([p], [z()], [(codes, scale)], [z()], 1), TypeError, "all float32"),
+            (([p], [z()], [(codes, z(2))], [(codes, scale)], 1), ValueError, "1 float32 scales"),
+            (([p], [z()], [(z(), scale)], [(codes, scale)], 1), TypeError, "float8"),
+    ]:
+        with pytest.raises(error, match=match):
+            adamw_step(*args)
+    with pytest.raises(ValueError, match="masters"):
+        adamw_step([p], [z()], [z()], [z()], 1, masters=[z()])
+    with pytest.raises(ValueError, match="lr as a tensor"):
+        adamw_step([p], [z()], [z()], [z()], 1, lr=torch.ones(1))
+    q = torch.nn.Parameter(p)
+    for kw in (dict(lr=-1), dict(betas=(1.0, 0.9)), dict(eps=-1), dict(weight_decay=-1), dict(state_bits=4),
+               dict(lr=torch.ones(1))):
+        with pytest.raises(ValueError):
+            AdamW([q], **kw)
+
+
+def test_adamw_c_entry_point_refuses_before_launching():
+    lib, one = capi.load(), 4096
+    row = lambda numel=4, master=0, scale=0: [numel, one, one, one, one, scale, scale, master]  # noqa: E731
+
+    def call(rows, **kw):
+        table = (C.c_int64 * (8 * max(1, len(rows))))(*[v for r in rows for v in r])
+        d = capi.AdamW(**{**dict(count=len(rows), state_bits=32, step=1, beta1=0.9, beta2=0.999), **kw})
+        d.tensors = C.addressof(table)
+        return lib.kvae_adamw_step(C.byref(d), None)
+
+    assert call([]) == -1 and call([row()] * 49) == -1 and call([row(0)]) == -1
+    assert call([row()], step=0) == -1 and call([row(), row(master=one)]) == -1
+    assert call([row()], state_bits=8) == -1                     # no scales
+    assert call([row()], state_bits=4) == -2 and call([row()], dtype=capi.KVAE_F64) == -2
+    assert lib.kvae_adamw_step(None, None) == -1
+    assert call([row(1 << 45)]) == -5
