@@ -773,6 +773,14 @@ int kvae_rms_norm_backward(const kvae_rms_norm *d, void *stream);
 int kvae_quantize_rows(int64_t rows, int64_t D, int dtype, const void *x, int64_t x_stride, void *q,
                        void *scale, void *stream);
 
+/* Product of 8-bit rows, y (M,N) = (x w^T) * x_scale[m] * w_scale[n] + bias[n]: the projection that
+ * reads kvae_rms_norm_quantized's output in the serving form of the "gated" network.  x (M,K) and
+ * w (N,K) contiguous e4m3 bytes at any address, x_scale (M), w_scale (N) and bias (N, or NULL) float;
+ * sums in float; y of out_dtype (KVAE_F32, KVAE_BF16 or KVAE_F16).  Any M, N, K >= 1.          */
+int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void *x, const void *x_scale,
+                     const void *w, const void *w_scale, const void *bias, int out_dtype, void *y,
+                     void *stream);
+
 /* ------------------------------------------------------------------------ */
 /* AdamW (decoupled weight decay) over up to KVAE_ADAMW_MAX_TENSORS tensors in one launch: the
  * optimiser step of a training loop (examples/train.py:126-131 steps torch.optim.Adam).

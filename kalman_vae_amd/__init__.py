@@ -11,7 +11,8 @@ from .state_space_model import StateSpaceModel
 from .elbo import kalman_elbo
 from .variational_autoencoder import BernoulliDecoder, Encoder, GaussianDecoder
 from .kalman_vae import KalmanVariationalAutoencoder
-from .sequence_ops import gated_scan, gated_scan_step, quantize_rows, rms_norm, rms_norm_quantized
+from .sequence_ops import (gated_scan, gated_scan_step, linear_8bit, quantize_rows, rms_norm,
+                           rms_norm_quantized)
 from .optim import AdamW, adamw_step
 from .functions import (kalman_filter_steps, kalman_smooth_steps, kalman_elbo_terms,
                         read_status)
@@ -20,4 +21,4 @@ __all__ = ["SampleControl", "aggregate", "LSTMModel", "MLPModel", "StateSpaceMod
            "kalman_elbo", "KalmanVariationalAutoencoder", "Encoder", "GaussianDecoder",
            "BernoulliDecoder", "kalman_filter_steps", "kalman_smooth_steps", "kalman_elbo_terms",
            "read_status", "gated_scan", "gated_scan_step", "rms_norm",
-           "rms_norm_quantized", "quantize_rows", "AdamW", "adamw_step"]
+           "rms_norm_quantized", "quantize_rows", "linear_8bit", "AdamW", "adamw_step"]

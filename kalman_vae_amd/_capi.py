@@ -127,6 +127,7 @@ EXPORTS = (
     "kvae_gated_scan_step",
     "kvae_rms_norm_backward_parts", "kvae_rms_norm_forward", "kvae_rms_norm_quantized",
     "kvae_rms_norm_backward", "kvae_quantize_rows", "kvae_adamw_step",
+    "kvae_linear_8bit",
 )
 
 
@@ -336,6 +337,8 @@ def load():
     lib.kvae_quantize_rows.restype = C.c_int
     lib.kvae_adamw_step.argtypes = [C.POINTER(AdamW), _vp]
     lib.kvae_adamw_step.restype = C.c_int
+    lib.kvae_linear_8bit.argtypes = [_i64] * 3 + [_vp] * 5 + [C.c_int, _vp, _vp]
+    lib.kvae_linear_8bit.restype = C.c_int
     _lib = lib
     return lib
 

@@ -1,0 +1,272 @@
+// Product of 8-bit rows on gfx950: y[m][n] = sx[m] sw[n] sum_k x[m][k] w[n][k] + bias[n], x and w in
+// e4m3 with one float scale per row (what rms_norm_quantized and quantize_rows write), summed in
+// float on the matrix instructions.
+//
+// 16-bit results take the instructions for 8-bit operands.  These add eight neighbouring products
+// aligned to the largest of them and drop what lies 2^-14 or more below it (seen by feeding them one
+// large and one small product, at every distance), 1.6e-5 of a sum of Gaussian terms: a hundredth of
+// a bfloat16 result's rounding and a fifteenth of a half's.  A float result would show it, so there
+// the bytes are widened to half, which holds every e4m3 value, and multiplied by the instructions for
+// half operands, at half the rate, whose sums are float throughout (1e-8 on the same terms).
+//
+// Both operands lie along k, so a lane's 32 operand bytes are contiguous in memory.  w takes the
+// first operand's place: then a lane's results are four neighbouring n of one row m, which go out
+// as one wide store, and the matrix instruction's k order does not matter as both sides share it.
+//
+// Two forms.  Few rows: reading w once is the work, so a workgroup takes 16 rows of w straight into
+// registers, its wavefronts share out k and add up through LDS.  Many rows: 128 x 128 tiles staged
+// through LDS, the next k slice on its way while the present one is multiplied.
+#include "narrow_types.h"
+
+namespace kvae {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+struct LinearArgs {
+    long M;
+    int N, K;
+    const uint8_t* x;
+    const uint8_t* w;
+    const float* sx;
+    const float* sw;
+    const float* bias;
+    void* y;
+};
+
+// 16 bytes of a row from byte k on; bytes at K and beyond, and rows that are not there, are zero.
+__device__ __forceinline__ v4i load_chunk(const uint8_t* row, bool there, int k, int K) {
+    v4i r = {0, 0, 0, 0};
+    if (there && k + 16 <= K) {
+        struct __attribute__((packed)) Any { v4i v; };
+        r = reinterpret_cast<const Any*>(row + k)->v;
+    } else if (there && k < K) {
+        for (int i = 0; k + i < K; ++i) {
+            const int b = (int)row[k + i] << (8 * (i & 3));
+            if (i < 4) r.x |= b; else if (i < 8) r.y |= b; else if (i < 12) r.z |= b; else r.w |= b;
+        }
+    }
+    return r;
+}
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// bytes 8 i .. 8 i + 7 of a lane's 32 as halves (exact)
+__device__ __forceinline__ v8h widen8(const v8i& a, int i) {
+    const v2h p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a[2 * i], 1.f, false);
+    const v2h q = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a[2 * i], 1.f, true);
+    const v2h r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a[2 * i + 1], 1.f, false);
+    const v2h t = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a[2 * i + 1], 1.f, true);
+    return v8h{p.x, p.y, q.x, q.y, r.x, r.y, t.x, t.y};
+}
+
+// whether results of this type need the products of widened operands
+template <typename T>
+constexpr bool WIDENED = sizeof(T) == 4;
+
+// four neighbouring results of one row
+template <typename T>
+__device__ __forceinline__ void store4(const LinearArgs& g, long m, int n, const float (&acc)[4]) {
+    if (m >= g.M || n >= g.N) return;
+    const float sx = g.sx[m];
+    T* out = static_cast<T*>(g.y) + m * g.N + n;
+    if (n + 4 <= g.N) {
+        const Pack<float, 4> sw = load_pack<float, 4>(g.sw + n);
+        Pack<float, 4> b{};
+        if (g.bias) b = load_pack<float, 4>(g.bias + n);
+        Pack<T, 4> p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.v[i] = narrow<T>(acc[i] * sx * sw.v[i] + b.v[i]);
+        store_pack<T, 4>(out, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < g.N) out[i] = narrow<T>(acc[i] * sx * g.sw[n + i] + (g.bias ? g.bias[n + i] : 0.f));
+    }
+}
+
+constexpr int FEW_WAVES = 8;
+// Rows of x: blockIdx.y * 16 MT ..., rows of w: blockIdx.x * 16 ...
+template <typename T, int MT>
+__global__ void __launch_bounds__(64 * FEW_WAVES) linear_few_rows_kernel(LinearArgs g) {
+    __shared__ float sums[FEW_WAVES][MT][64][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = lane & 15, part = (lane >> 4) * 32;
+    const long m0 = (long)blockIdx.y * 16 * MT;
+    const int n = blockIdx.x * 16 + row;
+    const bool has_n = n < g.N;
+    const uint8_t* w = g.w + (has_n ? (long)n * g.K : 0);
+    const uint8_t* x[MT];
+    bool has_m[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        has_m[t] = m0 + 16 * t + row < g.M;
+        x[t] = g.x + (has_m[t] ? (m0 + 16 * t + row) * (long)g.K : 0);
+    }
+    v4f acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = wave * 128; k0 < g.K; k0 += FEW_WAVES * 128) {
+        const int k = k0 + part;
+        const v4i a0 = load_chunk(w, has_n, k, g.K), a1 = load_chunk(w, has_n, k + 16, g.K);
+        const v8i a = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+        v8h ah[4];
+        if constexpr (WIDENED<T>) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ah[i] = widen8(a, i);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const v4i b0 = load_chunk(x[t], has_m[t], k, g.K), b1 = load_chunk(x[t], has_m[t], k + 16, g.K);
+            const v8i b = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+            if constexpr (WIDENED<T>) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[i], widen8(b, i), acc[t], 0, 0, 0);
+            } else {
+                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], 0, 0, 0, 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[wave][t][lane][i] = acc[t][i];
+    __syncthreads();
+    for (int t = wave; t < MT; t += FEW_WAVES) {
+        float total[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < FEW_WAVES; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[i] += sums[v][t][lane][i];
+        store4<T>(g, m0 + 16 * t + (lane & 15), blockIdx.x * 16 + 4 * (lane >> 4), total);
+    }
+}
+
+constexpr int TILE = 128, SLICE = 128;
+// LDS place of 16-byte piece c of row r: the exclusive-or spreads a column of pieces over the banks
+__device__ __forceinline__ int piece_at(int r, int c) { return r * (SLICE / 16) + (c ^ (r & 7)); }
+
+template <typename T>
+__global__ void __launch_bounds__(256) linear_tile_kernel(LinearArgs g) {
+    __shared__ v4i xs[TILE * SLICE / 16], ws[TILE * SLICE / 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long m0 = (long)blockIdx.y * TILE;
+    const int n0 = blockIdx.x * TILE;
+    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    v16f acc[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+    v4i xr[4], wr[4];
+    const auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = threadIdx.x + 256 * i, r = q >> 3, k = k0 + (q & 7) * 16;
+            xr[i] = load_chunk(g.x + (m0 + r) * g.K, m0 + r < g.M, k, g.K);
+            wr[i] = load_chunk(g.w + (long)(n0 + r) * g.K, n0 + r < g.N, k, g.K);
+        }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < g.K; k0 += SLICE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = threadIdx.x + 256 * i;
+            xs[piece_at(q >> 3, q & 7)] = xr[i];
+            ws[piece_at(q >> 3, q & 7)] = wr[i];
+        }
+        __syncthreads();
+        if (k0 + SLICE < g.K) fetch(k0 + SLICE);
+#pragma unroll
+        for (int s = 0; s < SLICE / 64; ++s) {
+            v8i a[2], b[2];
+            const int c = s * 4 + (lane >> 5) * 2;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int ra = wn + 32 * t + (lane & 31), rb = wm + 32 * t + (lane & 31);
+                const v4i p = ws[piece_at(ra, c)], q = ws[piece_at(ra, c + 1)];
+                a[t] = v8i{p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+                const v4i u = xs[piece_at(rb, c)], v = xs[piece_at(rb, c + 1)];
+                b[t] = v8i{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            }
+            if constexpr (WIDENED<T>) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const v8h bh[2] = {widen8(b[0], q), widen8(b[1], q)};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const v8h ah = widen8(a[i], q);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh[j], acc[i][j], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j],
+                                                                                    0, 0, 0, 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                                    acc[i][j][4 * q + 3]};
+                store4<T>(g, m0 + wm + 32 * j + (lane & 31), n0 + wn + 32 * i + 8 * q + 4 * (lane >> 5), v);
+            }
+}
+
+}  // namespace kvae
+
+using namespace kvae;
+
+extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scale,
+                                const void* w, const void* w_scale, const void* bias, int out_dtype,
+                                void* y, void* stream) {
+    if (M < 1 || N < 1 || K < 1 || !x || !x_scale || !w || !w_scale || !y) return KVAE_E_BADARG;
+    if (N > (1 << 30) || K > (1 << 30) || M > (1L << 38)) return KVAE_E_TOOLARGE;
+    return for_element_type(out_dtype, [&](auto e) {
+        using T = decltype(e);
+        const LinearArgs g{(long)M, (int)N, (int)K, static_cast<const uint8_t*>(x),
+                           static_cast<const uint8_t*>(w), static_cast<const float*>(x_scale),
+                           static_cast<const float*>(w_scale), static_cast<const float*>(bias), y};
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        if (M <= 64) {
+            const unsigned nb = (unsigned)((N + 15) / 16);
+            if (M <= 16) {
+                linear_few_rows_kernel<T, 1><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
+            } else if (M <= 32) {
+                linear_few_rows_kernel<T, 2><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
+            } else {
+                linear_few_rows_kernel<T, 4><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
+            }
+        } else {
+            const long my = (M + TILE - 1) / TILE;
+            // (blockIdx.y is 16 bits: rows beyond go in further launches)
+            for (long first = 0; first < my; first += 65535) {
+                LinearArgs h = g;
+                const long count = my - first < 65535 ? my - first : 65535;
+                h.M = g.M - first * TILE;
+                h.x = g.x + first * TILE * K;
+                h.sx = g.sx + first * TILE;
+                h.y = static_cast<T*>(y) + first * TILE * N;
+                linear_tile_kernel<T><<<dim3((unsigned)((N + TILE - 1) / TILE), (unsigned)count), 256, 0, s>>>(h);
+            }
+        }
+        return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
+    });
+}

@@ -1,6 +1,7 @@
 """Operators of the "gated" dynamics-parameter network, each on hand-written HIP kernels: the
 gated linear recurrence over a sequence and its one-step form (csrc/gated_scan.hip), the
-root-mean-square norm with the residual's addition and its 8-bit output (csrc/rms_norm.hip).
+root-mean-square norm with the residual's addition and its 8-bit output (csrc/rms_norm.hip),
+the product of 8-bit rows (csrc/linear_8bit.hip).
 
 They take GPU tensors of float32, bfloat16 or float16 and run on the current stream of the
 tensors' device; states, norms and sums are float32 whatever the element type.  The
@@ -361,3 +362,42 @@ def quantize_rows(x):
     elif D == 0:
         scale.fill_(2.0 ** -126)
     return q, scale
+
+
+def linear_8bit(x, x_scale, weight, weight_scale, bias=None, dtype=torch.float32):
+    """``y = (x * x_scale) (weight * weight_scale)^T + bias`` for 8-bit rows: x (..., K) with x_scale
+    (...) as ``rms_norm_quantized`` returns them, weight (N, K) with weight_scale (N) as
+    ``quantize_rows`` lays them out once; y (..., N) of ``dtype`` (float32, bfloat16 or float16).
+
+    The sum runs over the 8-bit values on the matrix instructions in float32; scales and bias
+    (float32) are applied before the one rounding to ``dtype``.  Any sizes.  Serving only: no
+    gradient."""
+    device = _device_of(x, x_scale, weight, weight_scale, bias)
+    code = capi.sequence_dtype_code(dtype)
+    for name, t in (("x", x), ("weight", weight)):
+        if t.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"{name} must be torch.float8_e4m3fn, got {t.dtype}")
+    for name, t in (("x_scale", x_scale), ("weight_scale", weight_scale), ("bias", bias)):
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32, got {t.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x (..., K) and weight (N, K) expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N, K = weight.shape
+    if x_scale.shape != x.shape[:-1] or tuple(weight_scale.shape) != (N,):
+        raise ValueError(f"one scale per row expected, got {tuple(x_scale.shape)} for x {tuple(x.shape)} and "
+                         f"{tuple(weight_scale.shape)} for weight {tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"bias must have shape {(N,)}, got {tuple(bias.shape)}")
+    _no_gradient("linear_8bit", x_scale, weight_scale, bias)
+    with _on(device):
+        y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=device)
+        if y.numel() == 0:
+            return y
+        if K == 0:
+            return y.copy_(bias) if bias is not None else y.zero_()
+        x, x_scale, weight, weight_scale = (t.contiguous() for t in (x, x_scale, weight, weight_scale))
+        bias = bias.contiguous() if bias is not None else None
+        capi.check(capi.load().kvae_linear_8bit(
+            x_scale.numel(), N, K, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
+            weight_scale.data_ptr(), capi.ptr(bias), code, y.data_ptr(), _stream(device)))
+    return y

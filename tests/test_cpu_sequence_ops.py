@@ -9,6 +9,10 @@ import kalman_vae_amd as kv
 from kalman_vae_amd import _capi as capi
 
 
+E8 = lambda *s: torch.zeros(s, dtype=torch.float8_e4m3fn)  # noqa: E731
+ONE = lambda *s: torch.ones(s)  # noqa: E731
+
+
 def test_no_cpu_path():
     u, w = torch.zeros(3, 2, 12), torch.ones(12)
     for call in (lambda: kv.gated_scan(u), lambda: kv.gated_scan_step(u[0], torch.zeros(2, 4)),
@@ -45,6 +49,15 @@ def as_if_on_gpu(monkeypatch):
     (lambda: kv.rms_norm_quantized(torch.zeros(3, 4), torch.ones(4, requires_grad=True)), RuntimeError, "no gradient"),
     (lambda: kv.quantize_rows(torch.zeros(3, 4, requires_grad=True)), RuntimeError, "no gradient"),
     (lambda: kv.quantize_rows(torch.zeros(1, 16385)), NotImplementedError, "16384"),
+    (lambda: kv.linear_8bit(torch.zeros(2, 4), ONE(2), E8(3, 4), ONE(3)), TypeError, "x must be"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(2), torch.zeros(3, 4), ONE(3)), TypeError, "weight must be"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(2).half(), E8(3, 4), ONE(3)), TypeError, "x_scale must be"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(2), E8(3, 5), ONE(3)), ValueError, "expected"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(3), E8(3, 4), ONE(3)), ValueError, "one scale per row"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(2), E8(3, 4), ONE(3, 1)), ValueError, "one scale per row"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(2), E8(3, 4), ONE(3), bias=ONE(4)), ValueError, "bias must have"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(2), E8(3, 4), ONE(3), dtype=torch.float64), TypeError, "float64"),
+    (lambda: kv.linear_8bit(E8(2, 4), ONE(2).requires_grad_(), E8(3, 4), ONE(3)), RuntimeError, "no gradient"),
 ])
 def test_refusals(monkeypatch, call, error, match):
     as_if_on_gpu(monkeypatch)
@@ -85,6 +98,10 @@ def test_c_entry_points_refuse_before_launching():
     assert lib.kvae_rms_norm_forward(C.byref(n), None) == -5
     assert lib.kvae_quantize_rows(2, 8, 1, one, 8, one, one, None) == -2
     assert lib.kvae_quantize_rows(2, 8, 0, one, 8, None, one, None) == -1
+    assert lib.kvae_linear_8bit(2, 8, 0, one, one, one, one, None, 0, one, None) == -1
+    assert lib.kvae_linear_8bit(2, 8, 4, one, None, one, one, None, 0, one, None) == -1
+    assert lib.kvae_linear_8bit(2, 8, 4, one, one, one, one, None, 1, one, None) == -2
+    assert lib.kvae_linear_8bit(2, 1 << 31, 4, one, one, one, one, None, 0, one, None) == -5
 
 
 def test_segments_of_the_time_axis():
