@@ -140,11 +140,6 @@ def ptr(t):
     return t.data_ptr()
 
 
-def ptr_strided(t):
-    """Device address of a tensor whose strides go with it; None -> NULL."""
-    return None if t is None else t.data_ptr()
-
-
 def fill(struct, **tensors):
     for k, v in tensors.items():
         if isinstance(v, int):
@@ -341,6 +336,29 @@ def load():
     lib.kvae_linear_8bit.restype = C.c_int
     _lib = lib
     return lib
+
+
+_torch_entry = None
+
+
+def torch_entry():
+    """The C++ module with the torch side of the sequence operators and the optimiser
+    (csrc/torch_entry.cpp), bound to the loaded library; raises if it has not been built."""
+    global _torch_entry
+    if _torch_entry is None:
+        import importlib.machinery
+        import importlib.util
+        path = os.path.join(_HERE, "csrc", "_torch_entry.so")
+        if not os.path.exists(path):
+            raise RuntimeError(
+                f"{path} not found: build it with `make -C kalman_vae_amd/csrc` "
+                "(or __graft_entry__.build()). kalman_vae_amd has no CPU fallback.")
+        loader = importlib.machinery.ExtensionFileLoader("_torch_entry", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_torch_entry", loader))
+        loader.exec_module(module)
+        module.bind(load()._handle)
+        _torch_entry = module
+    return _torch_entry
 
 
 def column_sum(x):

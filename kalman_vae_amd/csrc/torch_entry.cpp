@@ -1,0 +1,432 @@
+// Torch side of the sequence-network operators and of the optimiser: autograd nodes, output and
+// workspace allocation and the walk over tensor lists, in C++ so that a small call is not dominated
+// by the interpreter (a forward and backward call through Python functions took 130 us of host time
+// at 32 sequences, of which the kernels are 16 us; a list of 40 tensors 85 us).  All computing is in
+// the C ABI (include/kvae_kalman.h), whose addresses come from the library that Python has loaded.
+// The arguments' meaning is documented and checked in sequence_ops.py and optim.py.
+#include <dlfcn.h>
+
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <array>
+#include <unordered_set>
+#include <vector>
+
+#include "../../include/kvae_kalman.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+struct Library {
+    decltype(&kvae_error_string) error_string;
+    decltype(&kvae_gated_scan_workspace_bytes) scan_workspace_bytes;
+    decltype(&kvae_gated_scan_forward) scan_forward;
+    decltype(&kvae_gated_scan_backward) scan_backward;
+    decltype(&kvae_gated_scan_step) scan_step;
+    decltype(&kvae_rms_norm_forward) norm_forward;
+    decltype(&kvae_rms_norm_quantized) norm_quantized;
+    decltype(&kvae_rms_norm_backward) norm_backward;
+    decltype(&kvae_rms_norm_backward_parts) norm_parts;
+    decltype(&kvae_quantize_rows) quantize_rows;
+    decltype(&kvae_linear_8bit) linear_8bit;
+    decltype(&kvae_adamw_step) adamw_step;
+} lib;
+
+template <typename F>
+void find(void* handle, const char* name, F& f) {
+    f = reinterpret_cast<F>(dlsym(handle, name));
+    TORCH_CHECK(f, "the kernel library has no ", name);
+}
+
+void bind(uintptr_t address) {
+    void* handle = reinterpret_cast<void*>(address);
+    find(handle, "kvae_error_string", lib.error_string);
+    find(handle, "kvae_gated_scan_workspace_bytes", lib.scan_workspace_bytes);
+    find(handle, "kvae_gated_scan_forward", lib.scan_forward);
+    find(handle, "kvae_gated_scan_backward", lib.scan_backward);
+    find(handle, "kvae_gated_scan_step", lib.scan_step);
+    find(handle, "kvae_rms_norm_forward", lib.norm_forward);
+    find(handle, "kvae_rms_norm_quantized", lib.norm_quantized);
+    find(handle, "kvae_rms_norm_backward", lib.norm_backward);
+    find(handle, "kvae_rms_norm_backward_parts", lib.norm_parts);
+    find(handle, "kvae_quantize_rows", lib.quantize_rows);
+    find(handle, "kvae_linear_8bit", lib.linear_8bit);
+    find(handle, "kvae_adamw_step", lib.adamw_step);
+}
+
+void check(int code) { TORCH_CHECK(code == KVAE_OK, "kvae kernel call failed: ", lib.error_string(code)); }
+
+int dtype_code(at::ScalarType t) {
+    switch (t) {
+        case at::kFloat: return KVAE_F32;
+        case at::kBFloat16: return KVAE_BF16;
+        case at::kHalf: return KVAE_F16;
+        default: TORCH_CHECK_TYPE(false, "float32, bfloat16 or float16 expected, got ", t);
+    }
+}
+
+// The current stream of the tensor's device, which is made the current device meanwhile.
+struct On {
+    explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+    c10::DeviceGuard guard;
+    hipStream_t stream;
+};
+
+Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type) {
+    return at::empty(sizes, at::TensorOptions().dtype(type).device(like.device()));
+}
+Tensor empty(at::IntArrayRef sizes, const Tensor& like) { return empty(sizes, like, like.scalar_type()); }
+
+void* address(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
+
+Tensor rows_dense(const Tensor& t) {
+    return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
+// (rows, D) with last-axis stride 1; copies only when the leading axes do not merge
+Tensor as_rows(const Tensor& t, int64_t D) { return rows_dense(t).reshape({-1, D}); }
+
+// Gradients of a gradient are refused when they are asked for, not when the graph is built.
+variable_list once_differentiable(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto node = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that is differentiable once", (int64_t)grads.size());
+    for (auto& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    return (*node)(std::move(grads));
+}
+
+// -- gated recurrence -------------------------------------------------------------------------
+kvae_gated_scan scan_struct(const Tensor& u, const OptTensor& mask, bool gated) {
+    kvae_gated_scan d{};
+    d.T = u.size(0), d.B = u.size(1), d.H = u.size(2) / (gated ? 3 : 2);
+    d.dtype = dtype_code(u.scalar_type()), d.gated = gated;
+    d.u = u.data_ptr(), d.u_stride_t = u.stride(0), d.u_stride_b = u.stride(1);
+    if (mask && mask->defined()) {
+        d.mask = mask->data_ptr();
+        d.mask_stride_t = mask->stride(0), d.mask_stride_b = mask->stride(1);
+    }
+    return d;
+}
+
+Tensor scan_workspace(const kvae_gated_scan& d, const Tensor& like) {
+    return empty({(int64_t)lib.scan_workspace_bytes(d.T, d.B, d.H, d.dtype)}, like, at::kByte);
+}
+
+std::array<Tensor, 3> scan_forward(const Tensor& u, const OptTensor& h0, const OptTensor& mask, bool gated,
+                                   bool keep) {
+    const On on(u);
+    kvae_gated_scan d = scan_struct(u, mask, gated);
+    std::array<Tensor, 3> out = {empty({d.T, d.B, d.H}, u), empty({d.B, d.H}, u, at::kFloat), Tensor()};
+    if (keep) out[2] = empty({(d.T + KVAE_SCAN_CHUNK - 1) / KVAE_SCAN_CHUNK, d.B, d.H}, u, at::kFloat);
+    d.h0 = address(h0), d.y = out[0].data_ptr(), d.last = out[1].data_ptr();
+    d.states = keep ? out[2].data_ptr() : nullptr;
+    const Tensor ws = scan_workspace(d, u);
+    check(lib.scan_forward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream));
+    return out;
+}
+
+struct GatedScan : public torch::autograd::Function<GatedScan> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& u, const OptTensor& h0,
+                                 const OptTensor& mask, bool gated) {
+        auto out = scan_forward(u, h0, mask, gated, true);
+        ctx->save_for_backward({u, mask.value_or(Tensor()), out[2]});
+        ctx->saved_data["gated"] = gated;
+        ctx->saved_data["h0"] = h0.has_value();
+        ctx->set_materialize_grads(false);
+        return {out[0], out[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &u = saved[0], &mask = saved[1], &states = saved[2];
+        variable_list out(4);
+        {
+            at::AutoGradMode off(false);
+            const On on(u);
+            kvae_gated_scan d = scan_struct(u, mask, ctx->saved_data["gated"].toBool());
+            const Tensor dy = grads[0].defined() ? rows_dense(grads[0]) : at::zeros({d.T, d.B, d.H}, u.options());
+            const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+            out[0] = empty(u.sizes(), u);
+            if (ctx->saved_data["h0"].toBool()) out[1] = empty({d.B, d.H}, u, at::kFloat);
+            d.states = states.data_ptr();
+            d.dy = dy.data_ptr(), d.dy_stride_t = dy.stride(0), d.dy_stride_b = dy.stride(1);
+            d.dlast = address(dlast), d.du = out[0].data_ptr(), d.dh0 = address(out[1]);
+            const Tensor ws = scan_workspace(d, u);
+            check(lib.scan_backward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream));
+        }
+        return once_differentiable(std::move(out));
+    }
+};
+
+std::pair<Tensor, Tensor> gated_scan(const Tensor& u, const OptTensor& h0, const OptTensor& mask, bool gated) {
+    if (at::GradMode::is_enabled() && (u.requires_grad() || (h0 && h0->requires_grad()))) {
+        auto out = GatedScan::apply(rows_dense(u), h0 ? OptTensor(h0->contiguous()) : h0, mask, gated);
+        return {out[0], out[1]};
+    }
+    auto out = scan_forward(rows_dense(u), h0 ? OptTensor(h0->contiguous()) : h0, mask, gated, false);
+    return {out[0], out[1]};
+}
+
+Tensor gated_scan_step(const Tensor& u_in, const Tensor& state, const OptTensor& mask, bool gated) {
+    const Tensor u = rows_dense(u_in);
+    const On on(u);
+    const int64_t B = u.size(0), H = u.size(1) / (gated ? 3 : 2);
+    Tensor y = empty({B, H}, u);
+    check(lib.scan_step(B, H, dtype_code(u.scalar_type()), gated, u.data_ptr(), u.stride(0), address(mask),
+                        mask ? mask->stride(0) : 0, state.data_ptr(), y.data_ptr(), on.stream));
+    return y;
+}
+
+// -- norm -------------------------------------------------------------------------------------
+kvae_rms_norm norm_struct(const Tensor& x2, const Tensor& r2, const Tensor& weight, double eps) {
+    kvae_rms_norm d{};
+    d.rows = x2.size(0), d.D = x2.size(1);
+    d.dtype = dtype_code(x2.scalar_type()), d.weight_dtype = dtype_code(weight.scalar_type());
+    d.x = x2.data_ptr(), d.x_stride = x2.stride(0);
+    if (r2.defined()) d.residual = r2.data_ptr(), d.residual_stride = r2.stride(0);
+    d.weight = weight.data_ptr(), d.eps = (float)eps;
+    return d;
+}
+
+std::array<Tensor, 3> norm_forward(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps,
+                                   bool keep) {
+    const On on(x);
+    const int64_t D = x.size(-1);
+    const Tensor x2 = as_rows(x, D), r2 = residual ? as_rows(*residual, D) : Tensor();
+    std::array<Tensor, 3> out = {empty(x.sizes(), x), Tensor(), Tensor()};
+    if (residual) out[1] = empty(x.sizes(), x);
+    if (keep) out[2] = empty({x2.size(0)}, x, at::kFloat);
+    kvae_rms_norm d = norm_struct(x2, r2, weight, eps);
+    d.y = out[0].data_ptr(), d.sum = address(out[1]), d.rstd = address(out[2]);
+    check(lib.norm_forward(&d, on.stream));
+    return out;
+}
+
+struct RmsNorm : public torch::autograd::Function<RmsNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                                 const OptTensor& residual, double eps) {
+        auto out = norm_forward(x, weight, residual, eps, true);
+        // The backward pass forms the unrounded sum again from x and residual where the gradient of
+        // a float weight would show the 16-bit sum's rounding; elsewhere the stored sum serves (one
+        // tensor less to keep and to read).
+        const bool again = residual && x.scalar_type() != weight.scalar_type();
+        ctx->save_for_backward({residual && !again ? out[1] : x, again ? *residual : Tensor(), weight, out[2]});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["residual"] = residual.has_value();
+        ctx->set_materialize_grads(false);
+        return residual ? variable_list{out[0], out[1]} : variable_list{out[0]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &rstd = saved[3];
+        variable_list out(4);
+        {
+            at::AutoGradMode off(false);
+            const On on(x);
+            const int64_t D = x.size(-1);
+            const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(x.sizes(), x.options());
+            const Tensor dsum = grads.size() > 1 ? grads[1] : Tensor();
+            const Tensor x2 = as_rows(x, D), r2 = residual.defined() ? as_rows(residual, D) : Tensor();
+            const Tensor dy2 = as_rows(dy, D), ds2 = dsum.defined() ? as_rows(dsum, D) : Tensor();
+            out[0] = empty(x.sizes(), x);
+            out[1] = empty({D}, weight);
+            const Tensor partial = empty({lib.norm_parts(x2.size(0)), D}, x, at::kFloat);
+            kvae_rms_norm d = norm_struct(x2, r2, weight, ctx->saved_data["eps"].toDouble());
+            d.rstd = rstd.data_ptr(), d.dy = dy2.data_ptr(), d.dy_stride = dy2.stride(0);
+            if (ds2.defined()) d.dsum = ds2.data_ptr(), d.dsum_stride = ds2.stride(0);
+            d.dx = out[0].data_ptr(), d.partial = partial.data_ptr(), d.dweight = out[1].data_ptr();
+            check(lib.norm_backward(&d, on.stream));
+            if (ctx->saved_data["residual"].toBool()) out[2] = out[0];
+        }
+        return once_differentiable(std::move(out));
+    }
+};
+
+std::pair<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight_in, const OptTensor& residual,
+                                      double eps) {
+    const Tensor weight = weight_in.contiguous();
+    if (at::GradMode::is_enabled() &&
+        (x.requires_grad() || weight.requires_grad() || (residual && residual->requires_grad()))) {
+        auto out = RmsNorm::apply(x, weight, residual, eps);
+        return {out[0], residual ? OptTensor(out[1]) : OptTensor()};
+    }
+    auto out = norm_forward(x, weight, residual, eps, false);
+    return {out[0], residual ? OptTensor(out[1]) : OptTensor()};
+}
+
+std::tuple<Tensor, Tensor, OptTensor> rms_norm_quantized(const Tensor& x, const Tensor& weight_in,
+                                                         const OptTensor& residual, double eps) {
+    const On on(x);
+    const int64_t D = x.size(-1);
+    const Tensor weight = weight_in.contiguous(), x2 = as_rows(x, D);
+    const Tensor r2 = residual ? as_rows(*residual, D) : Tensor();
+    Tensor q = empty(x.sizes(), x, at::kFloat8_e4m3fn);
+    Tensor scale = empty(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
+    OptTensor sum;
+    if (residual) sum = empty(x.sizes(), x);
+    kvae_rms_norm d = norm_struct(x2, r2, weight, eps);
+    d.y = q.data_ptr(), d.scale = scale.data_ptr(), d.sum = address(sum);
+    check(lib.norm_quantized(&d, on.stream));
+    return {q, scale, sum};
+}
+
+std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
+    const On on(x);
+    const Tensor x2 = as_rows(x, x.size(-1));
+    Tensor q = empty(x.sizes(), x, at::kFloat8_e4m3fn);
+    Tensor scale = empty(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
+    check(lib.quantize_rows(x2.size(0), x2.size(1), dtype_code(x.scalar_type()), x2.data_ptr(), x2.stride(0),
+                            q.data_ptr(), scale.data_ptr(), on.stream));
+    return {q, scale};
+}
+
+Tensor linear_8bit(const Tensor& x_in, const Tensor& x_scale_in, const Tensor& w_in, const Tensor& w_scale_in,
+                   const OptTensor& bias_in, at::ScalarType dtype) {
+    const On on(x_in);
+    const Tensor x = x_in.contiguous(), xs = x_scale_in.contiguous(), w = w_in.contiguous(),
+                 ws = w_scale_in.contiguous();
+    const Tensor bias = bias_in ? bias_in->contiguous() : Tensor();
+    auto sizes = x.sizes().vec();
+    sizes.back() = w.size(0);
+    Tensor y = empty(sizes, x, dtype);
+    check(lib.linear_8bit(xs.numel(), w.size(0), w.size(1), x.data_ptr(), xs.data_ptr(), w.data_ptr(),
+                          ws.data_ptr(), address(bias), dtype_code(dtype), y.data_ptr(), on.stream));
+    return y;
+}
+
+// -- optimiser --------------------------------------------------------------------------------
+// The tensors of a Python list or tuple, borrowed from it (it holds them for the call).
+std::vector<const Tensor*> list_of(py::handle list, const char* name) {
+    TORCH_CHECK_TYPE(PyList_Check(list.ptr()) || PyTuple_Check(list.ptr()), name, ": a list of tensors is expected");
+    const auto seq = py::reinterpret_borrow<py::sequence>(list);
+    std::vector<const Tensor*> out;
+    out.reserve(seq.size());
+    for (const py::handle item : seq) {
+        TORCH_CHECK_TYPE(THPVariable_Check(item.ptr()), name, ": a list of tensors is expected");
+        out.push_back(&THPVariable_Unpack(item.ptr()));
+    }
+    return out;
+}
+
+bool is_pair(py::handle h) { return PyTuple_Check(h.ptr()) || PyList_Check(h.ptr()); }
+
+void check_list(const char* name, const std::vector<const Tensor*>& list, const std::vector<const Tensor*>& params,
+                at::ScalarType type, bool scales = false) {
+    TORCH_CHECK_VALUE(list.size() == params.size(), list.size(), " ", name, " for ", params.size(), " parameters");
+    for (size_t i = 0; i < list.size(); ++i) {
+        const Tensor &t = *list[i], &p = *params[i];
+        TORCH_CHECK_TYPE(t.scalar_type() == type, name, ": expected ", type, ", got ", t.scalar_type());
+        const int64_t want = scales ? (p.numel() + KVAE_ADAMW_BLOCK - 1) / KVAE_ADAMW_BLOCK : p.numel();
+        TORCH_CHECK_VALUE(t.numel() == want, name, ": ", want, scales ? " scales" : " elements",
+                          " expected for a parameter of ", p.numel(), " elements, got ", t.numel());
+        TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
+        TORCH_CHECK_VALUE(t.device() == p.device() && t.device() == params[0]->device(), name, " on ", t.device(),
+                          ", the first parameter on ", params[0]->device());
+    }
+}
+
+void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::object v_in, py::object step,
+                py::object lr, double beta1, double beta2, double eps, double weight_decay, py::object masters_in,
+                int64_t seed) {
+    const auto params = list_of(params_in, "parameters");
+    if (params.empty()) return;
+    const at::ScalarType type = params[0]->scalar_type();
+    kvae_adamw d{};
+    d.dtype = dtype_code(type);
+    check_list("parameters", params, params, type);
+    std::unordered_set<const void*> seen;
+    for (const Tensor* p : params)
+        TORCH_CHECK_VALUE(p->numel() == 0 || seen.insert(p->data_ptr()).second, "a parameter appears twice in the list");
+    const auto grads = list_of(grads_in, "gradients");
+    check_list("gradients", grads, params, type);
+    bool pairs = false, plain = false;
+    for (const auto& list : {m_in, v_in}) {
+        TORCH_CHECK_TYPE(is_pair(list), "states: lists are expected");
+        for (const py::handle item : py::reinterpret_borrow<py::sequence>(list)) (is_pair(item) ? pairs : plain) = true;
+    }
+    TORCH_CHECK_TYPE(!(pairs && plain), "states are all float32 tensors or all (codes, scales) pairs");
+    std::vector<const Tensor*> m, v, ms, vs, masters;
+    if (pairs) {
+        const auto split = [&](const py::object& list, const char* name, std::vector<const Tensor*>& codes,
+                               std::vector<const Tensor*>& scales) {
+            for (const py::handle item : py::reinterpret_borrow<py::sequence>(list)) {
+                const auto two = list_of(item, name);
+                TORCH_CHECK_TYPE(two.size() == 2, name, ": (codes, scales) pairs expected");
+                codes.push_back(two[0]);
+                scales.push_back(two[1]);
+            }
+            check_list(name, codes, params, at::kFloat8_e4m3fn);
+            check_list(name, scales, params, at::kFloat, true);
+        };
+        split(m_in, "exp_avgs", m, ms);
+        split(v_in, "exp_avg_sqs", v, vs);
+    } else {
+        check_list("exp_avgs", m = list_of(m_in, "exp_avgs"), params, at::kFloat);
+        check_list("exp_avg_sqs", v = list_of(v_in, "exp_avg_sqs"), params, at::kFloat);
+    }
+    if (!masters_in.is_none()) {
+        TORCH_CHECK_VALUE(type != at::kFloat, "masters belong to 16-bit parameters");
+        check_list("masters", masters = list_of(masters_in, "masters"), params, at::kFloat);
+    }
+    const Tensor& first = *params[0];
+    d.state_bits = pairs ? 8 : 32;
+    d.seed = (uint32_t)seed;
+    d.beta1 = beta1, d.beta2 = beta2, d.eps = eps, d.weight_decay = weight_decay;
+    const bool counted = THPVariable_Check(step.ptr());
+    if (counted) {
+        const Tensor& t = THPVariable_Unpack(step.ptr());
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.numel() == 1 && t.device() == first.device(),
+                          "step must be an int64 tensor of one element on the parameters' device");
+        d.step_device = t.data_ptr();
+    } else {
+        d.step = step.cast<int64_t>();
+        TORCH_CHECK_VALUE(d.step >= 1, "step counts from 1, got ", d.step);
+    }
+    if (THPVariable_Check(lr.ptr())) {
+        const Tensor& t = THPVariable_Unpack(lr.ptr());
+        TORCH_CHECK_VALUE(counted && t.scalar_type() == at::kFloat && t.numel() == 1 && t.device() == first.device(),
+                          "lr as a tensor: float32, one element, on the parameters' device, with step a tensor too");
+        d.lr_device = t.data_ptr();
+    } else {
+        d.lr = lr.cast<double>();
+    }
+    TORCH_CHECK(first.is_cuda(), "kalman_vae_amd runs on MI355X only: got a tensor on ", first.device(),
+                "; there is no CPU fallback");
+    const On on(first);
+    std::array<kvae_adamw_tensor, KVAE_ADAMW_MAX_TENSORS> table;
+    d.tensors = table.data();
+    int64_t blocks = 0;
+    const auto launch = [&] {
+        check(lib.adamw_step(&d, on.stream));
+        d.first_block += blocks;
+        d.count = 0, blocks = 0;
+    };
+    for (size_t i = 0; i < params.size(); ++i) {
+        const int64_t n = params[i]->numel();
+        if (n == 0) continue;
+        table[d.count++] = {n, params[i]->data_ptr(), grads[i]->data_ptr(), m[i]->data_ptr(), v[i]->data_ptr(),
+                            pairs ? ms[i]->data_ptr() : nullptr, pairs ? vs[i]->data_ptr() : nullptr,
+                            masters.empty() ? nullptr : masters[i]->data_ptr()};
+        blocks += (n + KVAE_ADAMW_BLOCK - 1) / KVAE_ADAMW_BLOCK;
+        if (d.count == KVAE_ADAMW_MAX_TENSORS) launch();
+    }
+    if (d.count) launch();
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("bind", &bind);
+    m.def("gated_scan", &gated_scan);
+    m.def("gated_scan_step", &gated_scan_step);
+    m.def("rms_norm", &rms_norm);
+    m.def("rms_norm_quantized", &rms_norm_quantized);
+    m.def("quantize_rows", &quantize_rows);
+    m.def("linear_8bit", &linear_8bit);
+    m.def("adamw_step", &adamw_step);
+}

@@ -4,37 +4,16 @@ model in one launch per 48 of them, with states in float32 or in 8 bits.
 The reference trains with torch.optim.Adam (examples/train.py:67, 126-131); ``AdamW`` here is used the same way, also
 in ``parallel.DataParallelStep``.
 """
-import ctypes as C
-
 import torch
 
 from . import _capi as capi
-from .sequence_ops import _on, _stream
 
 BLOCK = 256              # elements of an 8-bit state that share a scale
-MAX_TENSORS = 48         # tensors of one launch
 
 
 def state_blocks(numel):
     """Scales of an 8-bit state of `numel` elements."""
     return -(-numel // BLOCK)
-
-
-def _check_list(name, tensors, like, dtypes, device):
-    """Addresses of `tensors`: as many as `like`, of the same sizes, contiguous, on `device`."""
-    if len(tensors) != len(like):
-        raise ValueError(f"{len(tensors)} {name} for {len(like)} parameters")
-    for t, p in zip(tensors, like):
-        if t.dtype not in dtypes:
-            raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
-        if t.numel() != p.numel():
-            raise ValueError(f"{name}: {t.numel()} elements for a parameter of {p.numel()}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-        if t.device != device:
-            capi.require_gpu(t)
-            raise ValueError(f"{name} on {t.device}, parameters on {device}")
-    return [t.data_ptr() for t in tensors]
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
@@ -55,71 +34,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     ``step``: the number of this update, from 1; or an int64 tensor of one element on the device that
     holds it (then the call can be captured into a graph and replayed), in which case ``lr`` may be a
     float32 tensor of one element too.  Arithmetic is float32; nothing is allocated."""
-    if not params:
-        return
-    device, dtype = params[0].device, params[0].dtype
-    capi.require_gpu(params[0])
-    code = capi.sequence_dtype_code(dtype)
-    p_at = _check_list("parameters", params, params, (dtype,), device)
-    if len(set(p_at)) != len(p_at):
-        # (empty tensors have no address of their own and take no part)
-        full = [a for a, p in zip(p_at, params) if p.numel()]
-        if len(set(full)) != len(full):
-            raise ValueError("a parameter appears twice in the list")
-    g_at = _check_list("gradients", grads, params, (dtype,), device)
-    bits = 8 if exp_avgs and isinstance(exp_avgs[0], (tuple, list)) else 32
-    if any(isinstance(e, (tuple, list)) != (bits == 8) for e in (*exp_avgs, *exp_avg_sqs)):
-        raise TypeError("states are all float32 tensors or all (codes, scales) pairs")
-    if bits == 8:
-        code_types, f32 = (torch.float8_e4m3fn,), (torch.float32,)
-        columns = []
-        for name, pairs in (("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs)):
-            columns.append(_check_list(name, [c for c, _ in pairs], params, code_types, device))
-            scales = [s for _, s in pairs]
-            for s, p in zip(scales, params):
-                if s.dtype != torch.float32 or s.numel() != state_blocks(p.numel()):
-                    raise ValueError(f"{name}: {state_blocks(p.numel())} float32 scales for a parameter of "
-                                     f"{p.numel()}, got {s.numel()} of {s.dtype}")
-                if not s.is_contiguous() or s.device != device:
-                    raise ValueError(f"{name}: scales must be contiguous and on {device}")
-            columns.append([s.data_ptr() for s in scales])
-        m_at, ms_at, v_at, vs_at = columns
-    else:
-        m_at = _check_list("exp_avgs", exp_avgs, params, (torch.float32,), device)
-        v_at = _check_list("exp_avg_sqs", exp_avg_sqs, params, (torch.float32,), device)
-        ms_at = vs_at = [0] * len(params)
-    if masters is not None:
-        if dtype == torch.float32:
-            raise ValueError("masters belong to 16-bit parameters")
-        w_at = _check_list("masters", masters, params, (torch.float32,), device)
-    else:
-        w_at = [0] * len(params)
-    d = capi.AdamW(dtype=code, state_bits=bits, seed=int(seed) & 0xFFFFFFFF, beta1=betas[0], beta2=betas[1],
-                   eps=eps, weight_decay=weight_decay)
-    if isinstance(step, torch.Tensor):
-        if step.dtype != torch.int64 or step.numel() != 1 or step.device != device:
-            raise ValueError("step must be an int64 tensor of one element on the parameters' device")
-        d.step_device = step.data_ptr()
-    elif step < 1:
-        raise ValueError(f"step counts from 1, got {step}")
-    else:
-        d.step = step
-    if isinstance(lr, torch.Tensor):
-        if not isinstance(step, torch.Tensor) or lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
-            raise ValueError("lr as a tensor: float32, one element, on the parameters' device, with step a tensor too")
-        d.lr_device = lr.data_ptr()
-    else:
-        d.lr = lr
-    rows = [row for row in zip([p.numel() for p in params], p_at, g_at, m_at, v_at, ms_at, vs_at, w_at) if row[0]]
-    lib = capi.load()
-    with _on(device):
-        stream, first_block = _stream(device), 0
-        for i in range(0, len(rows), MAX_TENSORS):
-            part = rows[i:i + MAX_TENSORS]
-            table = (C.c_int64 * (8 * len(part)))(*[v for row in part for v in row])
-            d.tensors, d.count, d.first_block = C.addressof(table), len(part), first_block
-            capi.check(lib.kvae_adamw_step(C.byref(d), stream))
-            first_block += sum(-(-row[0] // BLOCK) for row in part)
+    capi.torch_entry().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, *betas, eps, weight_decay,
+                                  masters, int(seed) & 0xFFFFFFFF)
 
 
 class AdamW(torch.optim.Optimizer):

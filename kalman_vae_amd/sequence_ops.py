@@ -8,41 +8,24 @@ tensors' device; states, norms and sums are float32 whatever the element type.  
 reference's only recurrent network is torch.nn.LSTM (kvae/dynamics_parameter_network.py:18-58);
 these operators have no counterpart there.
 """
-import contextlib
-import ctypes as C
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _capi as capi
 
 
-def _device_of(*tensors):
+def _device_of(first, *others):
     """The one GPU all given tensors are on; raises for CPU tensors and for a mix."""
-    capi.require_gpu(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"tensors on different devices: {sorted(map(str, devices))}")
-    return devices.pop()
+    device = first.device
+    if not first.is_cuda:
+        capi.require_gpu(first)
+    for t in others:
+        if t is not None and t.device != device:
+            capi.require_gpu(t)
+            raise ValueError(f"tensors on different devices: {device} and {t.device}")
+    return device
 
 
-def _on(device):
-    """Context in which `device` is the current one (free when it already is)."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _rows_dense(t):
-    """`t` itself when its last axis has stride 1, a contiguous copy otherwise."""
-    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _mask_bytes(mask, shape, device_tensor):
+def _mask_bytes(mask, shape):
     """(T,B) or (B,) mask of any type as bytes (non-zero: the step counts), or None."""
     if mask is None:
         return None
@@ -71,71 +54,6 @@ def _state(h0, B, H, name):
     return h0
 
 
-def _scan_struct(u, mask, H, gated):
-    T, B = u.shape[:2]
-    d = capi.GatedScan(T=T, B=B, H=H, dtype=capi.sequence_dtype_code(u.dtype), gated=int(gated),
-                       u=u.data_ptr(), u_stride_t=u.stride(0), u_stride_b=u.stride(1))
-    if mask is not None:
-        d.mask, d.mask_stride_t, d.mask_stride_b = mask.data_ptr(), mask.stride(0), mask.stride(1)
-    return d
-
-
-def _scan_workspace(lib, d, device):
-    size = lib.kvae_gated_scan_workspace_bytes(d.T, d.B, d.H, d.dtype)
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
-
-
-def _scan_forward(u, h0, mask, gated, keep):
-    """(y, last, states): states, what the backward pass starts its chunks from, only if `keep`."""
-    lib, (T, B) = capi.load(), u.shape[:2]
-    H = u.shape[2] // (3 if gated else 2)
-    with _on(u.device):
-        y = torch.empty(T, B, H, dtype=u.dtype, device=u.device)
-        last = torch.empty(B, H, dtype=torch.float32, device=u.device)
-        states = torch.empty(-(-T // capi.SCAN_CHUNK) if keep else 0, B, H, dtype=torch.float32,
-                             device=u.device)
-        d = _scan_struct(u, mask, H, gated)
-        d.h0, d.y, d.last = capi.ptr(h0), y.data_ptr(), last.data_ptr()
-        d.states = states.data_ptr() if keep else None
-        ws = _scan_workspace(lib, d, u.device)
-        capi.check(lib.kvae_gated_scan_forward(C.byref(d), capi.ptr(ws), ws.numel() if ws is not None else 0,
-                                               _stream(u.device)))
-    return y, last, states
-
-
-class GatedScanFunction(torch.autograd.Function):
-    """(u, h0, mask bytes, gated) -> (y, last state)."""
-
-    @staticmethod
-    def forward(ctx, u, h0, mask, gated):
-        y, last, states = _scan_forward(u, h0, mask, gated, keep=True)
-        ctx.save_for_backward(u, mask, states)
-        ctx.gated, ctx.has_h0 = gated, h0 is not None
-        ctx.set_materialize_grads(False)
-        return y, last
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dlast):
-        u, mask, states = ctx.saved_tensors
-        lib, (T, B) = capi.load(), u.shape[:2]
-        H = u.shape[2] // (3 if ctx.gated else 2)
-        with _on(u.device):
-            dy = torch.zeros(T, B, H, dtype=u.dtype, device=u.device) if dy is None else _rows_dense(dy)
-            dlast = dlast.contiguous() if dlast is not None else None
-            du = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-            dh0 = torch.empty(B, H, dtype=torch.float32, device=u.device) if ctx.has_h0 else None
-            d = _scan_struct(u, mask, H, ctx.gated)
-            d.states, d.dy, d.dlast = states.data_ptr(), dy.data_ptr(), capi.ptr(dlast)
-            d.dy_stride_t, d.dy_stride_b = dy.stride(0), dy.stride(1)
-            d.du, d.dh0 = du.data_ptr(), capi.ptr(dh0)
-            ws = _scan_workspace(lib, d, u.device)
-            capi.check(lib.kvae_gated_scan_backward(C.byref(d), capi.ptr(ws),
-                                                    ws.numel() if ws is not None else 0,
-                                                    _stream(u.device)))
-        return du, dh0, None, None
-
-
 def gated_scan(u, h0=None, mask=None, output_gate=True):
     """Gated linear recurrence over a sequence: ``(y (T,B,H), last state (B,H) float32)``.
 
@@ -161,16 +79,11 @@ def gated_scan(u, h0=None, mask=None, output_gate=True):
     T, B = u.shape[:2]
     H = _scan_width(u, output_gate)
     h0 = _state(h0, B, H, "h0")
-    mask = _mask_bytes(mask, (T, B), u)
+    mask = _mask_bytes(mask, (T, B))
     if u.numel() == 0:
         last = h0.clone() if h0 is not None else torch.zeros(B, H, dtype=torch.float32, device=u.device)
         return u[..., :H].clone(), last       # (empty, connected to u)
-    u = _rows_dense(u)
-    h0 = h0.contiguous() if h0 is not None else None
-    if torch.is_grad_enabled() and (u.requires_grad or (h0 is not None and h0.requires_grad)):
-        return GatedScanFunction.apply(u, h0, mask, bool(output_gate))
-    y, last, _ = _scan_forward(u, h0, mask, output_gate, keep=False)
-    return y, last
+    return capi.torch_entry().gated_scan(u, h0, mask, bool(output_gate))
 
 
 def gated_scan_step(u, state, mask=None, output_gate=True):
@@ -178,10 +91,10 @@ def gated_scan_step(u, state, mask=None, output_gate=True):
     contiguous, is updated in place.  ``mask`` (B): a sequence whose entry is zero keeps its state and
     gets y = 0.  One launch, one pass over u, state and y.  Records no gradient and refuses to run
     where one would be lost."""
-    device = _device_of(u, state, mask)
+    _device_of(u, state, mask)
     if u.dim() != 2:
         raise ValueError(f"u must have shape (B, parts * H), got {tuple(u.shape)}")
-    code = capi.sequence_dtype_code(u.dtype)
+    capi.sequence_dtype_code(u.dtype)
     B, H = u.shape[0], _scan_width(u, output_gate)
     _state(state, B, H, "state")
     if not state.is_contiguous():
@@ -189,32 +102,15 @@ def gated_scan_step(u, state, mask=None, output_gate=True):
     if torch.is_grad_enabled() and (u.requires_grad or state.requires_grad):
         raise RuntimeError("gated_scan_step records no gradient: call it under torch.no_grad(), or "
                            "gated_scan on a sequence of one step")
-    mask = _mask_bytes(mask, (B,), u)
+    mask = _mask_bytes(mask, (B,))
     if u.numel() == 0:
         return u.new_zeros(B, H)
-    u = _rows_dense(u)
-    with _on(device):
-        y = torch.empty(B, H, dtype=u.dtype, device=device)
-        capi.check(capi.load().kvae_gated_scan_step(
-            B, H, code, int(output_gate), u.data_ptr(), u.stride(0), capi.ptr_strided(mask),
-            mask.stride(0) if mask is not None else 0, state.data_ptr(), y.data_ptr(), _stream(device)))
-    return y
+    return capi.torch_entry().gated_scan_step(u, state, mask, bool(output_gate))
 
 
 # -- root-mean-square norm ------------------------------------------------------------------
-def _rows(t, D):
-    """`t` as (rows, D) with last-axis stride 1; copies only when its leading axes do not merge."""
-    if t is None:
-        return None
-    t = _rows_dense(t)
-    try:
-        return t.view(-1, D)
-    except RuntimeError:
-        return t.reshape(-1, D)
-
-
 def _check_norm(x, weight, residual):
-    device = _device_of(x, weight, residual)
+    _device_of(x, weight, residual)
     capi.sequence_dtype_code(x.dtype)
     if x.dim() < 1:
         raise ValueError("x must have at least one axis")
@@ -229,68 +125,6 @@ def _check_norm(x, weight, residual):
         raise TypeError(f"residual must have x's type {x.dtype}, got {residual.dtype}")
     if D > capi.NORM_MAX_WIDTH:
         raise NotImplementedError(f"rows of up to {capi.NORM_MAX_WIDTH} elements, got {D}")
-    return device
-
-
-def _norm_struct(x2, r2, weight, eps):
-    d = capi.RmsNorm(rows=x2.shape[0], D=x2.shape[1], dtype=capi.sequence_dtype_code(x2.dtype),
-                     weight_dtype=capi.sequence_dtype_code(weight.dtype), x=x2.data_ptr(),
-                     x_stride=x2.stride(0), weight=weight.data_ptr(), eps=eps)
-    if r2 is not None:
-        d.residual, d.residual_stride = r2.data_ptr(), r2.stride(0)
-    return d
-
-
-def _norm_forward(x, weight, residual, eps, keep):
-    """(y, sum or None, rstd or None), the first two shaped like x."""
-    D = x.shape[-1]
-    x2, r2 = _rows(x, D), _rows(residual, D)
-    with _on(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r2 is not None else None
-        rstd = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device) if keep else None
-        d = _norm_struct(x2, r2, weight, eps)
-        d.y, d.sum, d.rstd = y.data_ptr(), capi.ptr(total), capi.ptr(rstd)
-        capi.check(capi.load().kvae_rms_norm_forward(C.byref(d), _stream(x.device)))
-    return y, total, rstd
-
-
-class RmsNormFunction(torch.autograd.Function):
-    """(x, weight, residual or None, eps) -> y, or (y, sum) with a residual."""
-
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        y, total, rstd = _norm_forward(x, weight, residual, eps, keep=True)
-        # The backward pass forms the unrounded sum again from x and residual where the gradient of
-        # a float32 weight would show the 16-bit sum's rounding; elsewhere the stored sum serves
-        # (one tensor less to keep and to read).
-        again = residual is not None and x.dtype != weight.dtype
-        ctx.save_for_backward(x if total is None or again else total, residual if again else None,
-                              weight, rstd)
-        ctx.eps, ctx.has_residual = eps, residual is not None
-        ctx.set_materialize_grads(False)
-        return y if total is None else (y, total)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dsum=None):
-        x, residual, weight, rstd = ctx.saved_tensors
-        lib, D = capi.load(), x.shape[-1]
-        with _on(x.device):
-            dy = torch.zeros_like(x) if dy is None else dy
-            x2, r2, dy2, ds2 = _rows(x, D), _rows(residual, D), _rows(dy, D), _rows(dsum, D)
-            rows = x2.shape[0]
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            dweight = torch.empty(D, dtype=weight.dtype, device=x.device)
-            partial = torch.empty(lib.kvae_rms_norm_backward_parts(rows), D, dtype=torch.float32,
-                                  device=x.device)
-            d = _norm_struct(x2, r2, weight, ctx.eps)
-            d.rstd, d.dy, d.dy_stride = rstd.data_ptr(), dy2.data_ptr(), dy2.stride(0)
-            if ds2 is not None:
-                d.dsum, d.dsum_stride = ds2.data_ptr(), ds2.stride(0)
-            d.dx, d.partial, d.dweight = dx.data_ptr(), partial.data_ptr(), dweight.data_ptr()
-            capi.check(lib.kvae_rms_norm_backward(C.byref(d), _stream(x.device)))
-        return dx, dweight, dx if ctx.has_residual else None, None
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
@@ -307,10 +141,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
         r = x if residual is None else x + residual
         y = r * weight.to(x.dtype)
         return y if residual is None else (y, r)
-    weight = weight.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
-        return RmsNormFunction.apply(x, weight, residual, float(eps))
-    y, total, _ = _norm_forward(x, weight, residual, float(eps), keep=False)
+    y, total = capi.torch_entry().rms_norm(x, weight, residual, eps)
     return y if residual is None else (y, total)
 
 
@@ -324,44 +155,32 @@ def rms_norm_quantized(x, weight, residual=None, eps=1e-6):
     residual.  q has x's shape in torch.float8_e4m3fn and scale x's leading shape in float32:
     ``y ~ q * scale[..., None]`` with ``scale = max(max |y| / 448, 2^-126)`` per row, to the nearest.
     A NaN stays one and does not enter the scale.  Serving only: no gradient."""
-    device = _check_norm(x, weight, residual)
+    _check_norm(x, weight, residual)
     _no_gradient("rms_norm_quantized", x, weight, residual)
-    D = x.shape[-1]
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
-    total = torch.empty(x.shape, dtype=x.dtype, device=device) if residual is not None else None
     if x.numel():
-        x2, r2, weight = _rows(x, D), _rows(residual, D), weight.contiguous()
-        with _on(device):
-            d = _norm_struct(x2, r2, weight, float(eps))
-            d.y, d.scale, d.sum = q.data_ptr(), scale.data_ptr(), capi.ptr(total)
-            capi.check(capi.load().kvae_rms_norm_quantized(C.byref(d), _stream(device)))
-    elif D == 0:
-        scale.fill_(2.0 ** -126)
+        q, scale, total = capi.torch_entry().rms_norm_quantized(x, weight, residual, eps)
+    else:
+        (q, scale), total = _empty_quantized(x), x if residual is None else x + residual
     return (q, scale) if residual is None else (q, scale, total)
+
+
+def _empty_quantized(x):
+    return (torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device),
+            torch.full(x.shape[:-1], 2.0 ** -126, dtype=torch.float32, device=x.device))
 
 
 def quantize_rows(x):
     """The last axis of x in 8 bits with one scale per row: ``(q, scale)`` as in
     ``rms_norm_quantized`` without the norm.  Lays out the weights of ``linear_8bit`` once."""
-    device = _device_of(x)
-    code = capi.sequence_dtype_code(x.dtype)
+    _device_of(x)
+    capi.sequence_dtype_code(x.dtype)
     if x.dim() < 1:
         raise ValueError("x must have at least one axis")
     D = x.shape[-1]
     if D > capi.NORM_MAX_WIDTH:
         raise NotImplementedError(f"rows of up to {capi.NORM_MAX_WIDTH} elements, got {D}")
     _no_gradient("quantize_rows", x)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
-    if x.numel():
-        x2 = _rows(x, D)
-        with _on(device):
-            capi.check(capi.load().kvae_quantize_rows(x2.shape[0], D, code, x2.data_ptr(), x2.stride(0),
-                                                      q.data_ptr(), scale.data_ptr(), _stream(device)))
-    elif D == 0:
-        scale.fill_(2.0 ** -126)
-    return q, scale
+    return capi.torch_entry().quantize_rows(x) if x.numel() else _empty_quantized(x)
 
 
 def linear_8bit(x, x_scale, weight, weight_scale, bias=None, dtype=torch.float32):
@@ -372,8 +191,8 @@ def linear_8bit(x, x_scale, weight, weight_scale, bias=None, dtype=torch.float32
     The sum runs over the 8-bit values on the matrix instructions in float32; scales and bias
     (float32) are applied before the one rounding to ``dtype``.  Any sizes.  Serving only: no
     gradient."""
-    device = _device_of(x, x_scale, weight, weight_scale, bias)
-    code = capi.sequence_dtype_code(dtype)
+    _device_of(x, x_scale, weight, weight_scale, bias)
+    capi.sequence_dtype_code(dtype)
     for name, t in (("x", x), ("weight", weight)):
         if t.dtype != torch.float8_e4m3fn:
             raise TypeError(f"{name} must be torch.float8_e4m3fn, got {t.dtype}")
@@ -389,15 +208,7 @@ def linear_8bit(x, x_scale, weight, weight_scale, bias=None, dtype=torch.float32
     if bias is not None and tuple(bias.shape) != (N,):
         raise ValueError(f"bias must have shape {(N,)}, got {tuple(bias.shape)}")
     _no_gradient("linear_8bit", x_scale, weight_scale, bias)
-    with _on(device):
-        y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=device)
-        if y.numel() == 0:
-            return y
-        if K == 0:
-            return y.copy_(bias) if bias is not None else y.zero_()
-        x, x_scale, weight, weight_scale = (t.contiguous() for t in (x, x_scale, weight, weight_scale))
-        bias = bias.contiguous() if bias is not None else None
-        capi.check(capi.load().kvae_linear_8bit(
-            x_scale.numel(), N, K, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
-            weight_scale.data_ptr(), capi.ptr(bias), code, y.data_ptr(), _stream(device)))
-    return y
+    if x_scale.numel() == 0 or N == 0 or K == 0:
+        y = torch.zeros(x.shape[:-1] + (N,), dtype=dtype, device=x.device)
+        return y if bias is None else y + bias.to(dtype)
+    return capi.torch_entry().linear_8bit(x, x_scale, weight, weight_scale, bias, dtype)
