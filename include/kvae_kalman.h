@@ -700,10 +700,10 @@ int kvae_graph_count_kernel_nodes(void *hip_graph);
  * needs the element's alignment only.  y (T,B,H), du (T,B,3H or 2H), h0, last, dlast, dh0 (B,H)
  * are contiguous and must not overlap the inputs.
  * forward: writes y, last = c_{T-1} (or NULL) and, for a later backward call, states
- *   (ceil(T / KVAE_SCAN_CHUNK), B, H): c before every KVAE_SCAN_CHUNK-th step (or NULL).
+ *   (ceil(T / L), B, H): c before every L-th step, L = KVAE_SCAN_CHUNK(dtype) (or NULL).
  * backward: reads u, mask, states, dy and dlast (or NULL); writes du and dh0 (or NULL).
  * Both need kvae_gated_scan_workspace_bytes() bytes (0 unless the time axis is split).       */
-#define KVAE_SCAN_CHUNK 16
+#define KVAE_SCAN_CHUNK(dtype) ((dtype) == KVAE_F32 ? 16 : 8)
 typedef struct {
     int64_t T, B, H;
     int32_t dtype;

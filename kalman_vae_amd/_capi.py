@@ -14,7 +14,6 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("KVAE_LIB_PATH") or os.path.join(_HERE, "csrc", "libkvae_kalman.so")
 
 KVAE_F32, KVAE_F64, KVAE_BF16, KVAE_F16 = 0, 1, 2, 3
-SCAN_CHUNK = 16
 OP_FILTER_BWD, OP_SMOOTH_BWD, OP_ELBO_BWD, OP_LOSS_FWD, OP_LOSS_BWD = 1, 2, 3, 4, 5
 OP_LOSS_VALUE_AND_GRAD = 6
 

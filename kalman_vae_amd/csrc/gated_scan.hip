@@ -4,28 +4,32 @@
 //
 // element-wise over (B,H): unlike the LSTM's recurrence there is no matrix product between steps,
 // so the work is a stream over memory: the forward pass reads u = [x | forget | o] and writes y,
-// the backward pass reads u and dy and writes du.
+// the backward pass reads u and dy and writes du.  The state is float whatever the element type.
 //
-// Mapping: a lane owns one channel (float) or two neighbouring ones (16-bit types) of one
-// sequence, so that a wavefront moves 256 contiguous bytes per tensor and step, and walks its
-// steps in chunks of CHUNK: the loads of a whole chunk are issued before the first is used.
-// The state stays in registers in float, whatever the element type.
+// Mapping.  A lane owns one channel (float) or two neighbouring ones (16-bit types) of one
+// sequence, so that a wavefront moves 256 contiguous bytes per tensor and step.  It takes its steps
+// in chunks (16 float, 8 16-bit), loads a whole chunk before using it, and keeps what a step needs
+// in registers: f and (1 - f) x.  With many channels a wavefront walks over the sequence alone.
+// With fewer, the four wavefronts of a workgroup take four consecutive chunks of the same channels
+// at once: each composes its chunk to c_out = P c_in + S in registers, the compositions meet in LDS,
+// and every wavefront then runs its chunk from its own start state, so that u is still read once.
+// Only when even that does not fill the card is the sequence cut into segments for several
+// workgroups: a launch that composes each segment, then the same kernel, which folds the
+// compositions of the segments before its own into its start state.
 //
 // The backward pass does not read y (which is rounded to the element type, and gated): the
 // forward pass leaves the float state before every chunk, and the backward pass runs a chunk's
 // recurrence again from there in registers, on the x and forget it has to read anyway.
 //
-// When B*H lanes do not fill the card, the time axis is cut into segments of whole chunks: one
-// launch composes each segment's steps to c_out = P c_in + S, a second composes the segments, and
-// the main kernel starts every segment from its state.
+// Bound by memory.  1000 steps of 4096 x 64 float channels: 4.2 GB in 0.86 ms forward and 7.3 GB in
+// 1.46 ms backward, 4.9 and 5.0 TB/s, where a large copy reaches 5.1.
 #include "narrow_types.h"
-
-#include "device_info.h"
 
 namespace kvae {
 
-constexpr int CHUNK = KVAE_SCAN_CHUNK;   // steps whose loads are in flight together
 constexpr int SCAN_BLOCK = 256;
+constexpr int TOGETHER = 4;                  // wavefronts that share a stretch of time
+constexpr int MOST_SEGMENTS = 128;
 
 struct ScanArgs {
     long T, B, H;
@@ -43,327 +47,497 @@ struct ScanArgs {
     void* du;
     float* dh0;
     long groups;                 // lanes per sequence
-    long seg;                    // steps per segment, a multiple of CHUNK
-    long segs;
+    long seg;                    // steps per segment, a multiple of the chunk
+    int segs;
     float2* compose;             // (segs, B, H): P and S of each segment
-    float* carry;                // (segs, B, H): state a segment starts from
 };
+
+// exp(z) from the hardware's 2^x: the argument is rounded once, the result within an ulp
+__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * 1.44269504f); }
 
 struct Gate {
-    float f, keep;               // sigmoid(z), 1 - sigmoid(z), both without cancellation
+    float f, keep;               // sigmoid(z), 1 - sigmoid(z), both without cancellation; NaN stays
 };
 __device__ __forceinline__ Gate sigmoid_pair(float z) {
-    const float e = __expf(-fabsf(z));
+    const float e = exp_of(-fabsf(z));
     const float big = __builtin_amdgcn_rcpf(1.f + e);
     const float small = e * big;
-    return z >= 0.f ? Gate{big, small} : (z < 0.f ? Gate{small, big} : Gate{z, z});
+    return z >= 0.f ? Gate{big, small} : Gate{small, big};
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_of(-z)); }
+
+// A lane's place: sequence b0 + b with b0 the workgroup's first, channels h .. h + V - 1.  Addresses
+// are a uniform base (scalar registers, moved from step to step by scalar instructions) plus a
+// 32-bit lane offset that stays: 64-bit lane pointers would be kept for every step and tensor and
+// take more registers than the data.
+// The last lane of a sequence is moved back so that its V channels end at H, and lanes behind the
+// last sequence repeat its last lane (so that a workgroup stays whole): a channel that two lanes own
+// gets the same values from both.
+struct Place {
+    long b0;
+    unsigned b, h;
+};
+template <int V, int W>
+__device__ __forceinline__ Place scan_place(const ScanArgs& g) {
+    const long first = (long)blockIdx.x * (W == 1 ? SCAN_BLOCK : 64);
+    Place p;
+    p.b0 = first / g.groups;
+    const long left = g.B * g.groups - first;        // lanes from here to the last one
+    unsigned lane = W == 1 ? threadIdx.x : threadIdx.x & 63;
+    if (lane >= left) lane = (unsigned)left - 1;
+    const unsigned groups = (unsigned)g.groups, inside = (unsigned)(first - p.b0 * g.groups) + lane;
+    p.b = inside / groups;
+    p.h = (inside - p.b * groups) * V;
+    if (p.h > (unsigned)g.H - V) p.h = (unsigned)g.H - V;
+    return p;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_off(const void* base, unsigned bytes) {
+    return load_pack<T, V>(reinterpret_cast<const T*>(static_cast<const char*>(base) + bytes));
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_off(void* base, unsigned bytes, const Pack<T, V>& x) {
+    store_pack<T, V>(reinterpret_cast<T*>(static_cast<char*>(base) + bytes), x);
 }
 
-// Lane -> (sequence, first channel).  The last lane of a sequence is moved back so that its V
-// channels end at H: a channel that two lanes own gets the same values from both.
 template <int V>
-__device__ __forceinline__ bool scan_lane(const ScanArgs& g, long& b, long& h) {
-    const long c = (long)blockIdx.x * SCAN_BLOCK + threadIdx.x;
-    if (c >= g.B * g.groups) return false;
-    b = c / g.groups;
-    h = (c - b * g.groups) * V;
-    if (h > g.H - V) h = g.H - V;
-    return true;
+struct Map {                     // c -> P c + S
+    float P[V], S[V];
+};
+template <int V>
+__device__ __forceinline__ Map<V> identity() {
+    Map<V> m;
+#pragma unroll
+    for (int v = 0; v < V; ++v) m.P[v] = 1.f, m.S[v] = 0.f;
+    return m;
+}
+// first `a`, then `b`
+template <int V>
+__device__ __forceinline__ Map<V> then(const Map<V>& a, const Map<V>& b) {
+    Map<V> m;
+#pragma unroll
+    for (int v = 0; v < V; ++v) m.P[v] = a.P[v] * b.P[v], m.S[v] = b.P[v] * a.S[v] + b.S[v];
+    return m;
 }
 
-template <typename T, int V, bool GATED, bool MASKED>
-__global__ void __launch_bounds__(SCAN_BLOCK) scan_forward_kernel(ScanArgs g) {
-    long b, h;
-    if (!scan_lane<V>(g, b, h)) return;
+// What the wavefronts of a workgroup tell each other: one map per wavefront and lane.
+template <int V, int W>
+struct Exchange {
+    Map<V> m[W][64];
+};
+
+// State (or, REVERSE, gradient) that segment blockIdx.y starts from: `init`, then the maps of the
+// segments that come before it in walking order.  With several wavefronts each takes every W-th of
+// them in one stretch and the stretches meet in LDS.
+template <int V, int W, bool REVERSE>
+__device__ __forceinline__ void segment_start(const ScanArgs& g, int wave, long at, const float* init, Exchange<V, W>* ex,
+                                              float (&c)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = init ? init[at + v] : 0.f;
+    if (g.segs == 1) return;
+    const long plane = g.B * g.H;
+    const int before = REVERSE ? g.segs - 1 - (int)blockIdx.y : (int)blockIdx.y;
+    const int each = (before + W - 1) / W;
+    const int begin = wave * each < before ? wave * each : before;
+    const int end = begin + each < before ? begin + each : before;
+    Map<V> m = identity<V>();
+#pragma unroll 8
+    for (int i = begin; i < end; ++i) {
+        const float2* p = g.compose + (REVERSE ? g.segs - 1 - i : i) * plane + at;
+        Map<V> k;
+#pragma unroll
+        for (int v = 0; v < V; ++v) k.P[v] = p[v].x, k.S[v] = p[v].y;
+        m = then<V>(m, k);
+    }
+    if constexpr (W > 1) {
+        ex->m[wave][threadIdx.x & 63] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const Map<V> k = ex->m[w][threadIdx.x & 63];
+#pragma unroll
+            for (int v = 0; v < V; ++v) c[v] = k.P[v] * c[v] + k.S[v];
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = m.P[v] * c[v] + m.S[v];
+    }
+}
+
+// Chunks come in two forms of the same code.  FULL: all L steps are there.  Otherwise n of them are
+// (possibly none): the loads of the others repeat the last step of the segment, so that they stay
+// inside the tensors, and count as masked, so that no load waits behind a branch.
+
+// The scheduler works step by step: left alone it computes all steps of a chunk side by side, which
+// takes several times the registers (and spills) for no gain, as other wavefronts fill the gaps.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// p + by, a scalar address the compiler takes as new: it would otherwise work out the addresses of
+// all steps of all tensors ahead of the loop and run out of scalar registers.
+template <typename P>
+__device__ __forceinline__ P* move_on(P* p, long by) {
+    p += by;
+    asm("" : "+s"(p));
+    return p;
+}
+
+// A loaded word, unpacked from here on and not before (unpacked 16-bit pairs take twice the registers).
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> now(const Pack<T, V>& x) {
+    if constexpr (sizeof(x) == 4) {
+        unsigned word = __builtin_bit_cast(unsigned, x);
+        asm volatile("" : "+v"(word));
+        return __builtin_bit_cast(Pack<T, V>, word);
+    } else {
+        return x;
+    }
+}
+
+// A value computed here and not where it is used (what it is computed from would be kept instead).
+__device__ __forceinline__ void settle(float& x) { asm volatile("" : "+v"(x)); }
+
+// Steps t0 .. t0 + L - 1 of the lane's channels: x, forget, output gate and, BACKWARD, dy.
+template <typename T, int V, int L, bool GATED, bool MASKED, bool FULL, bool WITH_X, bool WITH_GATE, bool WITH_DY>
+__device__ __forceinline__ void load_steps(const ScanArgs& g, const Place& at, long t0, long t_end, int n,
+                                           Pack<T, V> (&x)[L], Pack<T, V> (&z)[L], Pack<T, V> (&o)[L],
+                                           Pack<T, V> (&d)[L], bool (&live)[L]) {
+    const long t = FULL || t0 < t_end ? t0 : t_end - 1;
+    const T* p = static_cast<const T*>(g.u) + at.b0 * g.u_b + t * g.u_t;
+    const T* q = WITH_DY ? static_cast<const T*>(g.dy) + at.b0 * g.dy_b + t * g.dy_t : nullptr;
+    const uint8_t* m = MASKED ? g.mask + t * g.mask_t + at.b0 * g.mask_b : nullptr;
+    const unsigned pu = (at.b * (unsigned)g.u_b + at.h) * (unsigned)sizeof(T);
+    const unsigned qu = WITH_DY ? (at.b * (unsigned)g.dy_b + at.h) * (unsigned)sizeof(T) : 0u;
+    const unsigned mu = MASKED ? at.b * (unsigned)g.mask_b : 0u;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+        if constexpr (WITH_X) x[i] = load_off<T, V>(p, pu);
+        z[i] = load_off<T, V>(p + g.H, pu);
+        if constexpr (GATED && WITH_GATE) o[i] = load_off<T, V>(p + 2 * g.H, pu);
+        if constexpr (WITH_DY) d[i] = load_off<T, V>(q, qu);
+        live[i] = FULL || i < n;
+        if constexpr (MASKED) live[i] = live[i] && m[mu] != 0;
+        const bool on = FULL || i + 1 < n;
+        p = move_on(p, on ? g.u_t : 0);
+        if constexpr (WITH_DY) q = move_on(q, on ? g.dy_t : 0);
+        if constexpr (MASKED) m = move_on(m, on ? g.mask_t : 0);
+    }
+    keep_order();
+}
+
+template <typename T, int V, int L, int W, bool GATED, bool MASKED>
+__global__ void __launch_bounds__(W == 1 ? SCAN_BLOCK : 64 * W, 4) scan_forward_kernel(ScanArgs g) {
+    __shared__ Exchange<V, W> ex[W == 1 ? 1 : 2];
+    const Place place = scan_place<V, W>(g);
+    const int lane = threadIdx.x & 63;
+    const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long t_begin = (long)blockIdx.y * g.seg;
     const long t_end = t_begin + g.seg < g.T ? t_begin + g.seg : g.T;
-    const long at = b * g.H + h, plane = g.B * g.H;
+    const long at = (place.b0 + place.b) * g.H + place.h, plane = g.B * g.H;
+    const long at0 = place.b0 * g.H;                 // at = at0 + place.b H + place.h
+    const unsigned inside = place.b * (unsigned)g.H + place.h;
     float c[V];
+    segment_start<V, W, false>(g, wave, at, g.h0, &ex[0], c);
+    int turn = 1;                                    // (segment_start has used ex[0])
+    const auto chunk = [&](auto full, long t0, int n) {
+        constexpr bool FULL = decltype(full)::value, SELECT = MASKED || !FULL;
+        Pack<T, V> x[L], z[L], o[L], none[L];
+        bool live[L];
+        load_steps<T, V, L, GATED, MASKED, FULL, true, true, false>(g, place, t0, t_end, n, x, z, o, none, live);
+        float f[L][V], add[L][V];
+        Map<V> own = identity<V>();
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-        c[v] = g.carry ? g.carry[blockIdx.y * plane + at + v] : (g.h0 ? g.h0[at + v] : 0.f);
-    const T* u = static_cast<const T*>(g.u) + b * g.u_b + h;
-    T* y = static_cast<T*>(g.y) + at;
-    for (long t0 = t_begin; t0 < t_end; t0 += CHUNK) {
-        const int n = t_end - t0 < CHUNK ? (int)(t_end - t0) : CHUNK;
-        if (g.states) {
-            float* s = g.states + (t0 / CHUNK) * plane + at;
+        for (int i = 0; i < L; ++i) {
+            const Pack<T, V> xi = now(x[i]), zi = now(z[i]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const Gate k = sigmoid_pair(widen(zi.v[v]));
+                f[i][v] = k.f;
+                add[i][v] = k.keep * widen(xi.v[v]);
+                if constexpr (SELECT) {
+                    f[i][v] = live[i] ? f[i][v] : 1.f;
+                    add[i][v] = live[i] ? add[i][v] : 0.f;
+                }
+                if constexpr (W > 1) {
+                    own.P[v] *= f[i][v];
+                    own.S[v] = f[i][v] * own.S[v] + add[i][v];
+                }
+            }
+            keep_order();
+        }
+        float s[V];
+        if constexpr (W > 1) {
+            Exchange<V, W>& e = ex[turn];
+            e.m[wave][lane] = own;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (w == wave) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) s[v] = c[v];
+                }
+                const Map<V> k = e.m[w][lane];
+#pragma unroll
+                for (int v = 0; v < V; ++v) c[v] = k.P[v] * c[v] + k.S[v];
+            }
+        } else {
 #pragma unroll
             for (int v = 0; v < V; ++v) s[v] = c[v];
         }
-        Pack<T, V> x[CHUNK], z[CHUNK], o[CHUNK];
-        bool live[CHUNK];
-        const T* p = u + t0 * g.u_t;
-        T* w = y + t0 * plane;
-        const uint8_t* m = MASKED ? g.mask + t0 * g.mask_t + b * g.mask_b : nullptr;
+        if (g.states && (FULL || n > 0)) {
+            Pack<float, V> q;
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            if (i < n) {
-                x[i] = load_pack<T, V>(p);
-                z[i] = load_pack<T, V>(p + g.H);
-                if constexpr (GATED) o[i] = load_pack<T, V>(p + 2 * g.H);
-                if constexpr (MASKED) live[i] = *m != 0, m += g.mask_t;
-                p += g.u_t;
+            for (int v = 0; v < V; ++v) q.v[v] = s[v];
+            store_off<float, V>(g.states + (t0 / L) * plane + at0, inside * 4u, q);
+        }
+        T* w = static_cast<T*>(g.y) + t0 * plane + at0;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            Pack<T, V> out, oi;
+            if constexpr (GATED) oi = now(o[i]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                s[v] = f[i][v] * s[v] + add[i][v];
+                float r = s[v];
+                if constexpr (GATED) {
+                    const float ov = widen(oi.v[v]);
+                    r = r * (ov * sigmoid(ov));
+                }
+                if constexpr (MASKED) r = live[i] ? r : 0.f;
+                out.v[v] = narrow<T>(r);
+            }
+            if (FULL || i < n) store_off<T, V>(w, inside * (unsigned)sizeof(T), out);
+            w = move_on(w, plane);
+            keep_order();
+        }
+        if constexpr (W == 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) c[v] = s[v];
+        } else {
+            // the sequence's last state comes from the wavefront that ran its last step
+            if (g.last && n > 0 && t0 + n == g.T) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) g.last[at + v] = s[v];
             }
         }
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            if (i < n) {
-                Pack<T, V> out;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const Gate k = sigmoid_pair(widen(z[i].v[v]));
-                    const float next = k.f * c[v] + k.keep * widen(x[i].v[v]);
-                    float r = next;
-                    if constexpr (GATED) {
-                        const float ov = widen(o[i].v[v]);
-                        r = next * (ov * sigmoid_pair(ov).f);
-                    }
-                    if constexpr (MASKED) {
-                        c[v] = live[i] ? next : c[v];
-                        r = live[i] ? r : 0.f;
-                    } else {
-                        c[v] = next;
-                    }
-                    out.v[v] = narrow<T>(r);
-                }
-                store_pack<T, V>(w, out);
-                w += plane;
-            }
+    };
+    // (which form a round of chunks takes is the same for the whole workgroup: it holds a barrier)
+    for (long base = t_begin; base < t_end; base += L * W, turn ^= 1) {
+        const long t0 = base + L * wave;
+        if (base + L * W <= t_end) {
+            chunk(std::true_type{}, t0, L);
+        } else {
+            chunk(std::false_type{}, t0, t_end - t0 >= L ? L : (t_end > t0 ? (int)(t_end - t0) : 0));
         }
     }
-    if (g.last && t_end == g.T) {
+    if (W == 1 && g.last && t_end == g.T) {
 #pragma unroll
         for (int v = 0; v < V; ++v) g.last[at + v] = c[v];
     }
 }
 
-// A segment's composition for the forward pass: c_out = P c_in + S.
-template <typename T, int V, bool MASKED>
-__global__ void __launch_bounds__(SCAN_BLOCK) scan_forward_compose_kernel(ScanArgs g) {
-    long b, h;
-    if (!scan_lane<V>(g, b, h)) return;
-    const long t_begin = (long)blockIdx.y * g.seg;
-    const long t_end = t_begin + g.seg < g.T ? t_begin + g.seg : g.T;
-    const long at = b * g.H + h, plane = g.B * g.H;
-    float P[V], S[V];
+// A segment's map, for the state (forward) or its gradient (BACKWARD): the workgroup's wavefronts
+// compose a stretch each, the first joins them.
+template <typename T, int V, int L, int W, bool GATED, bool MASKED, bool BACKWARD>
+__global__ void __launch_bounds__(64 * W) scan_compose_kernel(ScanArgs g) {
+    __shared__ Exchange<V, W> ex;
+    const Place place = scan_place<V, W>(g);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long t_first = (long)blockIdx.y * g.seg;
+    const long t_last = t_first + g.seg < g.T ? t_first + g.seg : g.T;
+    const long stretch = g.seg / W;                  // (a multiple of L)
+    const long t_begin = t_first + wave * stretch < t_last ? t_first + wave * stretch : t_last;
+    const long t_end = t_begin + stretch < t_last ? t_begin + stretch : t_last;
+    Map<V> own = identity<V>();
+    const auto chunk = [&](auto full, long t0, int n) {
+        constexpr bool FULL = decltype(full)::value, SELECT = MASKED || !FULL;
+        Pack<T, V> x[L], z[L], o[L], d[L];
+        bool live[L];
+        load_steps<T, V, L, GATED, MASKED, FULL, !BACKWARD, BACKWARD, BACKWARD>(g, place, t0, t_end, n, x, z, o, d,
+                                                                               live);
 #pragma unroll
-    for (int v = 0; v < V; ++v) P[v] = 1.f, S[v] = 0.f;
-    const T* u = static_cast<const T*>(g.u) + b * g.u_b + h;
-    for (long t0 = t_begin; t0 < t_end; t0 += CHUNK) {
-        const int n = t_end - t0 < CHUNK ? (int)(t_end - t0) : CHUNK;
-        Pack<T, V> x[CHUNK], z[CHUNK];
-        bool live[CHUNK];
-        const T* p = u + t0 * g.u_t;
-        const uint8_t* m = MASKED ? g.mask + t0 * g.mask_t + b * g.mask_b : nullptr;
+        for (int j = 0; j < L; ++j) {
+            const int i = BACKWARD ? L - 1 - j : j;
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            if (i < n) {
-                x[i] = load_pack<T, V>(p);
-                z[i] = load_pack<T, V>(p + g.H);
-                if constexpr (MASKED) live[i] = *m != 0, m += g.mask_t;
-                p += g.u_t;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            if (i < n) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const Gate k = sigmoid_pair(widen(z[i].v[v]));
-                    const float p = P[v] * k.f, s = k.f * S[v] + k.keep * widen(x[i].v[v]);
-                    if (!MASKED || live[i]) P[v] = p, S[v] = s;
+            for (int v = 0; v < V; ++v) {
+                const Gate k = sigmoid_pair(widen(z[i].v[v]));
+                float P, S;
+                if constexpr (BACKWARD) {            // carry -> f (dy silu(o) + carry)
+                    float dc = widen(d[i].v[v]);
+                    if constexpr (GATED) {
+                        const float ov = widen(o[i].v[v]);
+                        dc = dc * (ov * sigmoid(ov));
+                    }
+                    P = own.P[v] * k.f, S = k.f * (dc + own.S[v]);
+                } else {
+                    P = own.P[v] * k.f, S = k.f * own.S[v] + k.keep * widen(x[i].v[v]);
                 }
+                own.P[v] = !SELECT || live[i] ? P : own.P[v];
+                own.S[v] = !SELECT || live[i] ? S : own.S[v];
             }
+            keep_order();
+        }
+    };
+    const long chunks = (t_end - t_begin + L - 1) / L;
+    for (long k = 0; k < chunks; ++k) {
+        const long t0 = t_begin + (BACKWARD ? chunks - 1 - k : k) * L;
+        if (t_end - t0 >= L) {
+            chunk(std::true_type{}, t0, L);
+        } else {
+            chunk(std::false_type{}, t0, (int)(t_end - t0));
         }
     }
+    ex.m[wave][lane] = own;
+    __syncthreads();
+    if (wave != 0) return;
+    Map<V> all = ex.m[BACKWARD ? W - 1 : 0][lane];
 #pragma unroll
-    for (int v = 0; v < V; ++v) g.compose[blockIdx.y * plane + at + v] = make_float2(P[v], S[v]);
+    for (int w = 1; w < W; ++w) all = then<V>(all, ex.m[BACKWARD ? W - 1 - w : w][lane]);
+    const long at = (place.b0 + place.b) * g.H + place.h, plane = g.B * g.H;
+#pragma unroll
+    for (int v = 0; v < V; ++v) g.compose[blockIdx.y * plane + at + v] = make_float2(all.P[v], all.S[v]);
 }
 
 // Adjoint.  carry = f_{t+1} G_{t+1}, the gradient that reaches c_t from later steps:
 //   G_t = dy_t silu(o_t) + carry, dx = (1-f) G, dforget = f (1-f) (c_{t-1} - x) G, do = dy c silu'(o)
-template <typename T, int V, bool GATED, bool MASKED>
-__global__ void __launch_bounds__(SCAN_BLOCK) scan_backward_kernel(ScanArgs g) {
-    long b, h;
-    if (!scan_lane<V>(g, b, h)) return;
+// Everything but G is known once a chunk's states have been run again: do goes out at once, and a
+// step keeps f, dy silu(o), 1 - f and f (1-f) (c_{t-1} - x) until the gradient from behind is there.
+template <typename T, int V, int L, int W, bool GATED, bool MASKED>
+__global__ void __launch_bounds__(W == 1 ? SCAN_BLOCK : 64 * W, 4) scan_backward_kernel(ScanArgs g) {
+    __shared__ Exchange<V, W> ex[W == 1 ? 1 : 2];
+    const Place place = scan_place<V, W>(g);
+    const int lane = threadIdx.x & 63;
+    const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long t_begin = (long)blockIdx.y * g.seg;
     const long t_end = t_begin + g.seg < g.T ? t_begin + g.seg : g.T;
-    const long at = b * g.H + h, plane = g.B * g.H;
+    const long at = (place.b0 + place.b) * g.H + place.h, plane = g.B * g.H;
+    const long at0 = place.b0 * g.H;
+    const unsigned inside = place.b * (unsigned)g.H + place.h;
     const long row = (GATED ? 3 : 2) * g.H;
+    const unsigned du_inside = (place.b * (unsigned)row + place.h) * (unsigned)sizeof(T);
     float carry[V];
+    segment_start<V, W, true>(g, wave, at, g.dlast, &ex[0], carry);
+    int turn = 1;
+    const auto chunk = [&](auto full, long t0, int n) {
+        constexpr bool FULL = decltype(full)::value, SELECT = MASKED || !FULL;
+        Pack<T, V> x[L], z[L], o[L], d[L];
+        bool live[L];
+        float c[V];
+        const Pack<float, V> first =
+            load_off<float, V>(g.states + ((FULL || n > 0 ? t0 : t_end - 1) / L) * plane + at0, inside * 4u);
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-        carry[v] = g.carry ? g.carry[blockIdx.y * plane + at + v] : (g.dlast ? g.dlast[at + v] : 0.f);
-    const T* u = static_cast<const T*>(g.u) + b * g.u_b + h;
-    const T* dy = static_cast<const T*>(g.dy) + b * g.dy_b + h;
-    T* du = static_cast<T*>(g.du) + b * row + h;
-    for (long t0 = t_begin + ((t_end - t_begin - 1) / CHUNK) * CHUNK; t0 >= t_begin; t0 -= CHUNK) {
-        const int n = t_end - t0 < CHUNK ? (int)(t_end - t0) : CHUNK;
-        Pack<T, V> x[CHUNK], z[CHUNK], o[CHUNK], d[CHUNK];
-        float c[CHUNK][V], last[V];
-        bool live[CHUNK];
-        const float* s = g.states + (t0 / CHUNK) * plane + at;
+        for (int v = 0; v < V; ++v) c[v] = first.v[v];
+        load_steps<T, V, L, GATED, MASKED, FULL, true, true, true>(g, place, t0, t_end, n, x, z, o, d, live);
+        float f[L][V], keep[L][V], slope[L][V], into[L][V];
+        const long du_t = g.B * row;
+        T* w = static_cast<T*>(g.du) + t0 * du_t + place.b0 * row;
 #pragma unroll
-        for (int v = 0; v < V; ++v) last[v] = s[v];
-        const T* p = u + t0 * g.u_t;
-        const T* q = dy + t0 * g.dy_t;
-        const uint8_t* m = MASKED ? g.mask + t0 * g.mask_t + b * g.mask_b : nullptr;
+        for (int i = 0; i < L; ++i) {
+            Pack<T, V> dg, oi;
+            const Pack<T, V> xi = now(x[i]), zi = now(z[i]), di = now(d[i]);
+            if constexpr (GATED) oi = now(o[i]);
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            if (i < n) {
-                x[i] = load_pack<T, V>(p);
-                z[i] = load_pack<T, V>(p + g.H);
-                if constexpr (GATED) o[i] = load_pack<T, V>(p + 2 * g.H);
-                d[i] = load_pack<T, V>(q);
-                q += g.dy_t;
-                if constexpr (MASKED) live[i] = *m != 0, m += g.mask_t;
-                p += g.u_t;
+            for (int v = 0; v < V; ++v) {
+                const Gate k = sigmoid_pair(widen(zi.v[v]));
+                const float xv = widen(xi.v[v]);
+                const float next = k.f * c[v] + k.keep * xv;
+                float dc = widen(di.v[v]), go = 0.f;
+                if constexpr (GATED) {
+                    const float ov = widen(oi.v[v]);
+                    const Gate r = sigmoid_pair(ov);
+                    go = dc * next * (r.f * (1.f + ov * r.keep));
+                    dc = dc * (ov * r.f);
+                }
+                f[i][v] = k.f;
+                keep[i][v] = k.keep;
+                slope[i][v] = k.f * k.keep * (c[v] - xv);
+                into[i][v] = dc;
+                if constexpr (SELECT) {
+                    f[i][v] = live[i] ? k.f : 1.f;
+                    keep[i][v] = live[i] ? k.keep : 0.f;
+                    slope[i][v] = live[i] ? slope[i][v] : 0.f;
+                    into[i][v] = live[i] ? dc : 0.f;
+                    go = live[i] ? go : 0.f;
+                    c[v] = live[i] ? next : c[v];
+                } else {
+                    c[v] = next;
+                }
+                dg.v[v] = narrow<T>(go);
+                settle(f[i][v]), settle(keep[i][v]), settle(slope[i][v]), settle(into[i][v]);
             }
+            if constexpr (GATED) {
+                if (FULL || i < n) store_off<T, V>(w + 2 * g.H, du_inside, dg);
+            }
+            w = move_on(w, du_t);
+            keep_order();
         }
-        // c[i]: the state BEFORE step t0 + i
+        float a[V];
+        if constexpr (W > 1) {
+            Map<V> own = identity<V>();
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            if (i < n) {
+            for (int i = L - 1; i >= 0; --i) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    c[i][v] = last[v];
-                    const Gate k = sigmoid_pair(widen(z[i].v[v]));
-                    const float next = k.f * last[v] + k.keep * widen(x[i].v[v]);
-                    if (!MASKED || live[i]) last[v] = next;
+                    own.P[v] *= f[i][v];
+                    own.S[v] = f[i][v] * (into[i][v] + own.S[v]);
                 }
+                keep_order();
+            }
+            Exchange<V, W>& e = ex[turn];
+            e.m[wave][lane] = own;
+            __syncthreads();
+#pragma unroll
+            for (int k = W - 1; k >= 0; --k) {
+                if (k == wave) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) a[v] = carry[v];
+                }
+                const Map<V> r = e.m[k][lane];
+#pragma unroll
+                for (int v = 0; v < V; ++v) carry[v] = r.P[v] * carry[v] + r.S[v];
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) a[v] = carry[v];
+        }
+#pragma unroll
+        for (int i = L - 1; i >= 0; --i) {
+            w = move_on(w, -du_t);
+            Pack<T, V> dx, dz;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float G = into[i][v] + a[v];
+                dx.v[v] = narrow<T>(keep[i][v] * G);
+                dz.v[v] = narrow<T>(slope[i][v] * G);
+                a[v] = f[i][v] * G;
+            }
+            if (FULL || i < n) {
+                store_off<T, V>(w, du_inside, dx);
+                store_off<T, V>(w + g.H, du_inside, dz);
+            }
+            keep_order();
+        }
+        if constexpr (W == 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) carry[v] = a[v];
+        } else {
+            if (g.dh0 && t0 == 0) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) g.dh0[at + v] = a[v];
             }
         }
-        T* w = du + (t0 + n - 1) * g.B * row;
-#pragma unroll
-        for (int i = CHUNK - 1; i >= 0; --i) {
-            if (i < n) {
-                Pack<T, V> dx, dz, dg;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const Gate k = sigmoid_pair(widen(z[i].v[v]));
-                    const float xv = widen(x[i].v[v]), before = c[i][v];
-                    float dc = widen(d[i].v[v]), go = 0.f;
-                    if constexpr (GATED) {
-                        const float ov = widen(o[i].v[v]);
-                        const Gate q = sigmoid_pair(ov);
-                        const float now = k.f * before + k.keep * xv;
-                        go = dc * now * (q.f * (1.f + ov * q.keep));
-                        dc = dc * (ov * q.f);
-                    }
-                    const float G = dc + carry[v];
-                    float gx = k.keep * G, gz = k.f * k.keep * (before - xv) * G, on = k.f * G;
-                    if constexpr (MASKED) {
-                        gx = live[i] ? gx : 0.f;
-                        gz = live[i] ? gz : 0.f;
-                        go = live[i] ? go : 0.f;
-                        on = live[i] ? on : carry[v];
-                    }
-                    carry[v] = on;
-                    dx.v[v] = narrow<T>(gx);
-                    dz.v[v] = narrow<T>(gz);
-                    dg.v[v] = narrow<T>(go);
-                }
-                store_pack<T, V>(w, dx);
-                store_pack<T, V>(w + g.H, dz);
-                if constexpr (GATED) store_pack<T, V>(w + 2 * g.H, dg);
-                w -= g.B * row;
-            }
+    };
+    constexpr long SPAN = L * W;
+    for (long base = t_begin + ((t_end - t_begin - 1) / SPAN) * SPAN; base >= t_begin; base -= SPAN, turn ^= 1) {
+        const long t0 = base + L * wave;
+        if (base + SPAN <= t_end) {
+            chunk(std::true_type{}, t0, L);
+        } else {
+            chunk(std::false_type{}, t0, t_end - t0 >= L ? L : (t_end > t0 ? (int)(t_end - t0) : 0));
         }
     }
-    if (g.dh0 && t_begin == 0) {
+    if (W == 1 && g.dh0 && t_begin == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) g.dh0[at + v] = carry[v];
-    }
-}
-
-// A segment's composition for the backward pass: carry_out = P carry_in + S.
-template <typename T, int V, bool GATED, bool MASKED>
-__global__ void __launch_bounds__(SCAN_BLOCK) scan_backward_compose_kernel(ScanArgs g) {
-    long b, h;
-    if (!scan_lane<V>(g, b, h)) return;
-    const long t_begin = (long)blockIdx.y * g.seg;
-    const long t_end = t_begin + g.seg < g.T ? t_begin + g.seg : g.T;
-    const long at = b * g.H + h, plane = g.B * g.H;
-    float P[V], S[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) P[v] = 1.f, S[v] = 0.f;
-    const T* u = static_cast<const T*>(g.u) + b * g.u_b + h;
-    const T* dy = static_cast<const T*>(g.dy) + b * g.dy_b + h;
-    for (long t0 = t_begin + ((t_end - t_begin - 1) / CHUNK) * CHUNK; t0 >= t_begin; t0 -= CHUNK) {
-        const int n = t_end - t0 < CHUNK ? (int)(t_end - t0) : CHUNK;
-        Pack<T, V> z[CHUNK], o[CHUNK], d[CHUNK];
-        bool live[CHUNK];
-        const T* p = u + t0 * g.u_t;
-        const T* q = dy + t0 * g.dy_t;
-        const uint8_t* m = MASKED ? g.mask + t0 * g.mask_t + b * g.mask_b : nullptr;
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            if (i < n) {
-                z[i] = load_pack<T, V>(p + g.H);
-                if constexpr (GATED) o[i] = load_pack<T, V>(p + 2 * g.H);
-                d[i] = load_pack<T, V>(q);
-                q += g.dy_t;
-                if constexpr (MASKED) live[i] = *m != 0, m += g.mask_t;
-                p += g.u_t;
-            }
-        }
-#pragma unroll
-        for (int i = CHUNK - 1; i >= 0; --i) {
-            if (i < n) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const Gate k = sigmoid_pair(widen(z[i].v[v]));
-                    float dc = widen(d[i].v[v]);
-                    if constexpr (GATED) {
-                        const float ov = widen(o[i].v[v]);
-                        dc = dc * (ov * sigmoid_pair(ov).f);
-                    }
-                    const float p = k.f * P[v], s = k.f * (dc + S[v]);
-                    if (!MASKED || live[i]) P[v] = p, S[v] = s;
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) g.compose[blockIdx.y * plane + at + v] = make_float2(P[v], S[v]);
-}
-
-// State every segment starts from, in walking order (forward: first to last; backward: last to
-// first).  One workgroup has 64 channels; its 16 wavefronts share the segments, compose their own
-// stretch, exchange the compositions through LDS and walk the stretch again.
-constexpr int CARRY_WAVES = 16;
-template <bool REVERSE>
-__global__ void __launch_bounds__(64 * CARRY_WAVES)
-scan_carry_kernel(long channels, long segs, const float2* __restrict__ compose,
-                  const float* __restrict__ init, float* __restrict__ carry) {
-    __shared__ float2 stretch[CARRY_WAVES][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long c = (long)blockIdx.x * 64 + lane;
-    const bool in = c < channels;
-    const long each = (segs + CARRY_WAVES - 1) / CARRY_WAVES;
-    const long begin = wave * each < segs ? wave * each : segs;
-    const long end = begin + each < segs ? begin + each : segs;
-    float P = 1.f, S = 0.f;
-    if (in) {
-#pragma unroll 8
-        for (long i = begin; i < end; ++i) {
-            const float2 k = compose[(REVERSE ? segs - 1 - i : i) * channels + c];
-            S = k.x * S + k.y;
-            P *= k.x;
-        }
-    }
-    stretch[wave][lane] = make_float2(P, S);
-    __syncthreads();
-    if (!in) return;
-    float v = init ? init[c] : 0.f;
-    for (int w = 0; w < wave; ++w) v = stretch[w][lane].x * v + stretch[w][lane].y;
-#pragma unroll 8
-    for (long i = begin; i < end; ++i) {
-        const long s = REVERSE ? segs - 1 - i : i;
-        const float2 k = compose[s * channels + c];
-        carry[s * channels + c] = v;
-        v = k.x * v + k.y;
     }
 }
 
@@ -410,38 +584,57 @@ scan_step_kernel(long B, long H, const T* __restrict__ u, long u_b, const uint8_
     }
 }
 
-// Channels per lane: two 16-bit ones or one float make a dword per lane and load.
-template <typename T>
-int scan_width(long H) {
-    return sizeof(T) == 2 && H >= 2 ? 2 : 1;
-}
-
-// Segments of the time axis.  A wavefront keeps about 12 KB of loads in flight, so some 2000
-// wavefronts (two per SIMD) cover the memory's latency; with fewer channels the time axis is cut,
-// which reads part of the input twice: not before there are fewer than 512 wavefronts, and never
-// into segments of under two chunks.
-static long scan_segments(long T, long B, long H, int dtype) {
-    const long width = dtype != KVAE_F32 && H >= 2 ? 2 : 1;
-    const long waves = (B * ((H + width - 1) / width) + 63) / 64;
-    if (waves >= 512) return 1;
-    long segs = (2048 + waves - 1) / waves;
-    const long most = T / (2 * CHUNK);
-    if (segs > most) segs = most;
-    if (segs > 32768) segs = 32768;
-    return segs < 2 ? 1 : segs;
-}
-static long segment_steps(long T, long segs) {
-    const long each = (T + segs - 1) / segs;
-    return (each + CHUNK - 1) / CHUNK * CHUNK;
+// How the work is laid out, from the sizes alone (times: forward / backward, H = 128, us).
+// - 1024 wavefronts of channels or more (a SIMD has one): each walks over its sequence alone.  At
+//   1024 the two forms meet (float, T = 1000: 208/329 alone, 217/368 with four).
+// - Fewer: four wavefronts share the time axis, as long as there is more than one chunk.  At 256
+//   wavefronts and T = 1000: 57/90 against 135/210 alone; T = 20, 64 wavefronts: 4.4/6.8 against
+//   8.2/7.4.  (Eight: 5.1/8.7 there, and no faster on long sequences.)
+// - Fewer than 2048 with that: the sequence is cut into segments as well, up to 128, of at least two
+//   rounds of a workgroup each: 32768 steps of 520 half channels take 19 us to compose and 29 to
+//   run (one wavefront per segment and a launch for the start states: 47 + 10 + 54).  u is read
+//   twice then.
+struct Plan {
+    int V, L, W, segs;
+    long seg;                                        // steps per segment
+};
+static Plan scan_plan(long T, long B, long H, int dtype) {
+    Plan p;
+    p.V = dtype != KVAE_F32 && H >= 2 ? 2 : 1;
+    p.L = KVAE_SCAN_CHUNK(dtype);
+    const long waves = (B * ((H + p.V - 1) / p.V) + 63) / 64;
+    p.W = waves < 1024 && T > p.L ? TOGETHER : 1;
+    p.segs = 1;
+    p.seg = T;
+    const long round = (long)p.L * p.W;
+    if (p.W > 1 && waves * p.W < 2048 && T >= 4 * round) {
+        long want = (8192 + waves * p.W - 1) / (waves * p.W);
+        if (want > MOST_SEGMENTS) want = MOST_SEGMENTS;
+        if (want > T / (2 * round)) want = T / (2 * round);
+        const long each = ((T + want - 1) / want + round - 1) / round * round;
+        p.segs = (int)((T + each - 1) / each);
+        p.seg = each;
+    }
+    return p;
 }
 
 static int check_scan(const kvae_gated_scan* d) {
-    if (!d || d->T < 1 || d->B < 1 || d->H < 1 || !d->u || (d->mask && d->mask_stride_b < 0))
-        return KVAE_E_BADARG;
+    if (!d || d->T < 1 || d->B < 1 || d->H < 1 || !d->u) return KVAE_E_BADARG;
     if (d->dtype != KVAE_F32 && d->dtype != KVAE_BF16 && d->dtype != KVAE_F16)
         return KVAE_E_UNSUPPORTED;
-    // a workgroup holds 256 lanes and blockIdx.x is 31 bits
-    if (d->B > (1L << 38) / d->H) return KVAE_E_TOOLARGE;
+    // a workgroup holds at least 64 lanes and blockIdx.x is 31 bits
+    if (d->B > (1L << 36) / d->H) return KVAE_E_TOOLARGE;
+    // lane offsets are 32 bits: the sequences of a workgroup (up to 256 lanes of one channel) must
+    // lie within 2^31 bytes of each other
+    if (d->u_stride_b < 0 || d->dy_stride_b < 0 || d->mask_stride_b < 0) return KVAE_E_BADARG;
+    long sequences = 2L * SCAN_BLOCK / d->H + 2;     // (a lane owns at most two channels)
+    if (sequences > d->B) sequences = d->B;
+    const long size = d->dtype == KVAE_F32 ? 4 : 2, most = (1L << 31) / size;
+    const long stride = d->u_stride_b > d->dy_stride_b ? d->u_stride_b : d->dy_stride_b;
+    if (3 * d->H > most / (sequences + 1)) return KVAE_E_TOOLARGE;
+    if (sequences > 1 && (stride > (most - 3 * d->H) / (sequences - 1) ||
+                          d->mask_stride_b > (1L << 31) / (sequences - 1)))
+        return KVAE_E_TOOLARGE;
     return KVAE_OK;
 }
 
@@ -459,60 +652,49 @@ static ScanArgs scan_args(const kvae_gated_scan* d) {
     return g;
 }
 
-static void cut_time(ScanArgs& g, int dtype, void* workspace) {
-    const long segs = scan_segments(g.T, g.B, g.H, dtype);
-    g.seg = segment_steps(g.T, segs);
-    g.segs = (g.T + g.seg - 1) / g.seg;
-    if (g.segs > 1) {
-        g.compose = static_cast<float2*>(workspace);
-        g.carry = reinterpret_cast<float*>(g.compose + g.segs * g.B * g.H);
-    }
-}
-
-template <typename T, int V, bool BACKWARD, bool GATED, bool MASKED>
+template <typename T, int V, int W, bool BACKWARD, bool GATED, bool MASKED>
 static void launch_scan(ScanArgs g, hipStream_t stream) {
+    constexpr int L = KVAE_SCAN_CHUNK(sizeof(T) == 4 ? KVAE_F32 : KVAE_BF16);
+    constexpr int BLOCK = W == 1 ? SCAN_BLOCK : 64 * W, LANES = W == 1 ? SCAN_BLOCK : 64;
     g.groups = (g.H + V - 1) / V;
-    const dim3 grid((unsigned)((g.B * g.groups + SCAN_BLOCK - 1) / SCAN_BLOCK), (unsigned)g.segs);
-    if (g.segs > 1) {
-        const long channels = g.B * g.H;
-        const dim3 cgrid((unsigned)((channels + 63) / 64));
-        if constexpr (BACKWARD) {
-            scan_backward_compose_kernel<T, V, GATED, MASKED><<<grid, SCAN_BLOCK, 0, stream>>>(g);
-            scan_carry_kernel<true><<<cgrid, 64 * CARRY_WAVES, 0, stream>>>(channels, g.segs, g.compose,
-                                                                          g.dlast, g.carry);
-        } else {
-            scan_forward_compose_kernel<T, V, MASKED><<<grid, SCAN_BLOCK, 0, stream>>>(g);
-            scan_carry_kernel<false><<<cgrid, 64 * CARRY_WAVES, 0, stream>>>(channels, g.segs, g.compose,
-                                                                           g.h0, g.carry);
-        }
+    const dim3 grid((unsigned)((g.B * g.groups + LANES - 1) / LANES), (unsigned)g.segs);
+    if constexpr (W > 1) {
+        if (g.segs > 1)
+            scan_compose_kernel<T, V, L, W, BACKWARD && GATED, MASKED, BACKWARD><<<grid, BLOCK, 0, stream>>>(g);
     }
     if constexpr (BACKWARD)
-        scan_backward_kernel<T, V, GATED, MASKED><<<grid, SCAN_BLOCK, 0, stream>>>(g);
+        scan_backward_kernel<T, V, L, W, GATED, MASKED><<<grid, BLOCK, 0, stream>>>(g);
     else
-        scan_forward_kernel<T, V, GATED, MASKED><<<grid, SCAN_BLOCK, 0, stream>>>(g);
+        scan_forward_kernel<T, V, L, W, GATED, MASKED><<<grid, BLOCK, 0, stream>>>(g);
+}
+
+// f(std::bool_constant<x>{})
+template <typename F>
+static void with_bool(bool x, F&& f) {
+    x ? f(std::true_type{}) : f(std::false_type{});
 }
 
 template <bool BACKWARD>
 static int run_scan(const kvae_gated_scan* d, void* workspace, size_t bytes, hipStream_t stream) {
     if (bytes < kvae_gated_scan_workspace_bytes(d->T, d->B, d->H, d->dtype)) return KVAE_E_WORKSPACE;
+    const Plan plan = scan_plan(d->T, d->B, d->H, d->dtype);
+    ScanArgs g = scan_args(d);
+    g.seg = plan.seg, g.segs = plan.segs;
+    g.compose = static_cast<float2*>(workspace);
     return for_element_type(d->dtype, [&](auto e) {
         using T = decltype(e);
-        ScanArgs g = scan_args(d);
-        cut_time(g, d->dtype, workspace);
-        const auto go = [&](auto width, auto gated, auto masked) {
-            launch_scan<T, decltype(width)::value, BACKWARD, decltype(gated)::value,
-                        decltype(masked)::value>(g, stream);
-        };
-        const auto with_width = [&](auto gated, auto masked) {
-            if constexpr (sizeof(T) == 2) {
-                if (scan_width<T>(g.H) == 2) return go(std::integral_constant<int, 2>{}, gated, masked);
-            }
-            go(std::integral_constant<int, 1>{}, gated, masked);
-        };
-        const auto with_mask = [&](auto gated) {
-            g.mask ? with_width(gated, std::true_type{}) : with_width(gated, std::false_type{});
-        };
-        d->gated ? with_mask(std::true_type{}) : with_mask(std::false_type{});
+        with_bool(d->gated, [&](auto gated) {
+            with_bool(g.mask != nullptr, [&](auto masked) {
+                with_bool(plan.W > 1, [&](auto together) {
+                    constexpr int W = decltype(together)::value ? TOGETHER : 1;
+                    constexpr bool GATED = decltype(gated)::value, MASKED = decltype(masked)::value;
+                    if constexpr (sizeof(T) == 2) {
+                        if (plan.V == 2) return launch_scan<T, 2, W, BACKWARD, GATED, MASKED>(g, stream);
+                    }
+                    launch_scan<T, 1, W, BACKWARD, GATED, MASKED>(g, stream);
+                });
+            });
+        });
         return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
     });
 }
@@ -523,9 +705,8 @@ using namespace kvae;
 
 extern "C" size_t kvae_gated_scan_workspace_bytes(int64_t T, int64_t B, int64_t H, int dtype) {
     if (T < 1 || B < 1 || H < 1) return 0;
-    const long segs = scan_segments(T, B, H, dtype);
-    if (segs < 2) return 0;
-    return (size_t)segs * B * H * (sizeof(float2) + sizeof(float));
+    const Plan p = scan_plan(T, B, H, dtype);
+    return p.segs < 2 ? 0 : (size_t)p.segs * B * H * sizeof(float2);
 }
 
 extern "C" int kvae_gated_scan_forward(const kvae_gated_scan* d, void* workspace,

@@ -123,7 +123,8 @@ std::array<Tensor, 3> scan_forward(const Tensor& u, const OptTensor& h0, const O
     const On on(u);
     kvae_gated_scan d = scan_struct(u, mask, gated);
     std::array<Tensor, 3> out = {empty({d.T, d.B, d.H}, u), empty({d.B, d.H}, u, at::kFloat), Tensor()};
-    if (keep) out[2] = empty({(d.T + KVAE_SCAN_CHUNK - 1) / KVAE_SCAN_CHUNK, d.B, d.H}, u, at::kFloat);
+    const int64_t chunk = KVAE_SCAN_CHUNK(d.dtype);
+    if (keep) out[2] = empty({(d.T + chunk - 1) / chunk, d.B, d.H}, u, at::kFloat);
     d.h0 = address(h0), d.y = out[0].data_ptr(), d.last = out[1].data_ptr();
     d.states = keep ? out[2].data_ptr() : nullptr;
     const Tensor ws = scan_workspace(d, u);

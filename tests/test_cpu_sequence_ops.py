@@ -106,14 +106,15 @@ def test_c_entry_points_refuse_before_launching():
 
 def test_segments_of_the_time_axis():
     """The workspace says how the time axis is cut: not at all for short sequences or many channels,
-    and never into segments of fewer than two chunks."""
+    into at most 128 segments, none of fewer than two rounds of a workgroup (4 chunks of 8 or 16 steps)."""
     lib = capi.load()
     size = lambda T, B, H, d=0: lib.kvae_gated_scan_workspace_bytes(T, B, H, d)  # noqa: E731
-    assert size(1, 1, 1) == size(63, 1, 1) == size(1000, 4096, 128) == 0
-    for T in (64, 1000, 32768, 1 << 22):
+    assert size(1, 1, 1) == size(255, 1, 1) == size(127, 1, 1, 2) == size(1000, 4096, 128) == 0
+    for T in (256, 600, 1000, 32768, 1 << 22):
         for B, H, d in ((1, 1, 0), (1, 520, 3), (3, 65, 2)):
-            segs = size(T, B, H, d) / (12 * B * H)
-            assert segs == int(segs) and segs <= T / 32, (T, B, H, d)
+            segs = size(T, B, H, d) / (8 * B * H)
+            assert segs == int(segs) and segs <= min(128, T / (64 if d else 128)), (T, B, H, d)
+    assert size(1 << 22, 1, 1) == 128 * 8
 
 
 def test_ctypes_structs_match_header(tmp_path):
