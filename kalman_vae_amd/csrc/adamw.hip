@@ -16,7 +16,7 @@
 // - The code of a positive sqrt(v) is never zero: the update divides by it, and a zero under an m
 //   that was rounded up would make a step of a thousand times lr.
 // The arithmetic of the states is written without contraction into fused multiply-adds and with
-// correctly rounded roots and reciprocals: codes come out the same as from the formulas
+// correctly rounded roots and scales' reciprocals: codes come out the same as from the formulas
 // above evaluated one operation at a time.
 #include "narrow_types.h"
 
@@ -60,86 +60,89 @@ constexpr float E4M3_MAX = 448.f;
 constexpr float SMALLEST_SCALE = 1.17549435e-38f;    // smallest normal: its reciprocal is finite
 
 // Two rounds of multiply and shift (C. Wellons' 32-bit mix) over a multiplicative start.
-__device__ __forceinline__ unsigned random_bits(unsigned index, unsigned key) {
-    unsigned h = index * 0x9E3779B1u + key;
+constexpr unsigned INDEX_FACTOR = 0x9E3779B1u;
+__device__ __forceinline__ unsigned random_bits(unsigned h) {   // h = index * INDEX_FACTOR + key
     h = (h ^ (h >> 16)) * 0x7FEB352Du;
     h = (h ^ (h >> 15)) * 0x846CA68Bu;
     return h ^ (h >> 16);
 }
 
-// t >= 0 to an e4m3 value, up or down by 16 random bits; POSITIVE: never to zero unless t is.
+// x to an e4m3 byte, up or down by 16 random bits; POSITIVE (x >= 0): never to zero unless x is.
+// Where the value is normal in e4m3 (2^-6 and more) its three mantissa bits are the float's first
+// three: the random bits are added below them and cut off, and the exponent is moved from bias 127
+// to 7.  Below, the code counts steps of 2^-9.
 template <bool POSITIVE>
-__device__ __forceinline__ float round_e4m3(float t, unsigned random16) {
-    t = t > E4M3_MAX ? E4M3_MAX : t;                 // (a NaN stays)
-    const unsigned bits = __builtin_bit_cast(unsigned, t) + (random16 << 4) + 8u;
-    float normal = __builtin_bit_cast(float, bits & ~0xFFFFFu);
-    normal = normal > E4M3_MAX ? E4M3_MAX : normal;
-    float small = floorf(__fadd_rn(t * 512.f, ((float)random16 + 0.5f) * (1.f / 65536.f)));
-    if constexpr (POSITIVE) small = t > 0.f ? fmaxf(small, 1.f) : 0.f;
-    return t < 0.015625f ? small * (1.f / 512.f) : (t == t ? normal : t);
-}
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
-    int p = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
+__device__ __forceinline__ unsigned round_e4m3(float x, unsigned random16) {
+    const unsigned bits = __builtin_bit_cast(unsigned, x), size = bits & 0x7FFFFFFFu;
+    const float t = fabsf(x);
+    const unsigned normal = ((size + (random16 << 4) + 8u) >> 20) - (120u << 3);
+    unsigned small = (unsigned)__fadd_rn(t * 512.f, __builtin_fmaf((float)random16, 1.f / 65536.f, 0.5f / 65536.f));
+    if constexpr (POSITIVE) small = t > 0.f && small == 0u ? 1u : small;
+    unsigned code = t < 0.015625f ? small : normal;
+    code = code < 0x7Eu ? code : 0x7Eu;              // at most 448
+    code = t == t ? code : 0x7Fu;
+    return code | ((bits >> 24) & 0x80u);
 }
 
-template <typename T>
-__device__ __forceinline__ void load16(const T* p, int n, float (&x)[PER_LANE]) {
-    constexpr int V = 16 / sizeof(T);
-    if (n >= PER_LANE) {
+// A lane's 16 elements are four groups of four, 64 elements apart: 16 lanes hold a block of 256, and
+// every access of theirs is one contiguous run.  n: elements of the tensor from the lane's first on.
+constexpr int GROUP = 4, GROUPS = PER_LANE / GROUP, APART = 16 * GROUP;
+
+// FULL: all of the workgroup's elements are there.
+template <bool FULL, typename T>
+__device__ __forceinline__ void load16(const T* p, long n, float (&x)[PER_LANE]) {
 #pragma unroll
-        for (int i = 0; i < PER_LANE; i += V) {
-            const Pack<T, V> q = load_pack<T, V>(p + i);
+    for (int k = 0; k < GROUPS; ++k) {
+        if (FULL || n >= k * APART + GROUP) {
+            const Pack<T, GROUP> q = load_pack<T, GROUP>(p + k * APART);
 #pragma unroll
-            for (int v = 0; v < V; ++v) x[i + v] = widen(q.v[v]);
+            for (int v = 0; v < GROUP; ++v) x[k * GROUP + v] = widen(q.v[v]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < GROUP; ++v) x[k * GROUP + v] = k * APART + v < n ? widen(p[k * APART + v]) : 0.f;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) x[i] = i < n ? widen(p[i]) : 0.f;
     }
 }
-template <typename T>
-__device__ __forceinline__ void store16(T* p, int n, const float (&x)[PER_LANE]) {
-    constexpr int V = 16 / sizeof(T);
-    if (n >= PER_LANE) {
+template <bool FULL, typename T>
+__device__ __forceinline__ void store16(T* p, long n, const float (&x)[PER_LANE]) {
 #pragma unroll
-        for (int i = 0; i < PER_LANE; i += V) {
-            Pack<T, V> q;
+    for (int k = 0; k < GROUPS; ++k) {
+        if (FULL || n >= k * APART + GROUP) {
+            Pack<T, GROUP> q;
 #pragma unroll
-            for (int v = 0; v < V; ++v) q.v[v] = narrow<T>(x[i + v]);
-            store_pack<T, V>(p + i, q);
+            for (int v = 0; v < GROUP; ++v) q.v[v] = narrow<T>(x[k * GROUP + v]);
+            store_pack<T, GROUP>(p + k * APART, q);
+        } else {
+#pragma unroll
+            for (int v = 0; v < GROUP; ++v)
+                if (k * APART + v < n) p[k * APART + v] = narrow<T>(x[k * GROUP + v]);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (i < n) p[i] = narrow<T>(x[i]);
     }
 }
-// sixteen e4m3 bytes
-__device__ __forceinline__ void load_codes(const uint8_t* p, int n, float scale, float (&x)[PER_LANE]) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (n >= PER_LANE) {
-        struct __attribute__((packed)) Any { uint32_t w[4]; };
-        const Any a = *reinterpret_cast<const Any*>(p);
+// four e4m3 bytes at any address
+struct __attribute__((packed)) Word { uint32_t w; };
+template <bool FULL>
+__device__ __forceinline__ void load_codes(const uint8_t* p, long n, float scale, float (&x)[PER_LANE]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = a.w[i];
-    } else {
+    for (int k = 0; k < GROUPS; ++k) {
+        uint32_t w = 0;
+        if (FULL || n >= k * APART + GROUP) {
+            w = reinterpret_cast<const Word*>(p + k * APART)->w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (i < n) w[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(w[i], 0) * scale;
-        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(w[i], 1) * scale;
-        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(w[i], 2) * scale;
-        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(w[i], 3) * scale;
+            for (int v = 0; v < GROUP; ++v)
+                if (k * APART + v < n) w |= (uint32_t)p[k * APART + v] << (8 * v);
+        }
+        x[k * GROUP] = __builtin_amdgcn_cvt_f32_fp8(w, 0) * scale;
+        x[k * GROUP + 1] = __builtin_amdgcn_cvt_f32_fp8(w, 1) * scale;
+        x[k * GROUP + 2] = __builtin_amdgcn_cvt_f32_fp8(w, 2) * scale;
+        x[k * GROUP + 3] = __builtin_amdgcn_cvt_f32_fp8(w, 3) * scale;
     }
 }
 // Codes and scale of a block of 256 over a row of 16 lanes.  SHIFT: which half of the hash decides.
-template <bool POSITIVE, int SHIFT>
-__device__ __forceinline__ void store_codes(uint8_t* p, float* scale_at, bool first, int n,
-                                            const float (&x)[PER_LANE], unsigned index, unsigned key) {
+template <bool FULL, bool POSITIVE, int SHIFT>
+__device__ __forceinline__ void store_codes(uint8_t* p, float* scale_at, bool first, long n,
+                                            const float (&x)[PER_LANE], const unsigned (&random)[PER_LANE]) {
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) big = fmaxf(big, fabsf(x[i]));
@@ -147,28 +150,21 @@ __device__ __forceinline__ void store_codes(uint8_t* p, float* scale_at, bool fi
     const float scale = fmaxf(big * (1.f / E4M3_MAX), SMALLEST_SCALE);
     const float inverse = 1.f / scale;
     if (first) *scale_at = scale;
-    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float q[4];
+    for (int k = 0; k < GROUPS; ++k) {
+        uint32_t w = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float t = x[4 * i + k] * inverse;
-            const unsigned r = random_bits(index + 4 * i + k, key);
-            q[k] = copysignf(round_e4m3<POSITIVE>(fabsf(t), SHIFT ? r >> 16 : r & 0xFFFFu), t);
+        for (int v = 0; v < GROUP; ++v) {
+            const unsigned r = random[k * GROUP + v];
+            w |= round_e4m3<POSITIVE>(x[k * GROUP + v] * inverse, SHIFT ? r >> 16 : r & 0xFFFFu) << (8 * v);
         }
-        w[i] = pack_e4m3(q[0], q[1], q[2], q[3]);
-    }
-    if (n >= PER_LANE) {
-        struct __attribute__((packed)) Any { uint32_t w[4]; };
-        Any a;
+        if (FULL || n >= k * APART + GROUP) {
+            reinterpret_cast<Word*>(p + k * APART)->w = w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a.w[i] = w[i];
-        *reinterpret_cast<Any*>(p) = a;
-    } else {
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (i < n) p[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+            for (int v = 0; v < GROUP; ++v)
+                if (k * APART + v < n) p[k * APART + v] = (uint8_t)(w >> (8 * v));
+        }
     }
 }
 
@@ -198,50 +194,65 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const AdamArgs g) {
         if (g.first_chunk[mid] <= (int)blockIdx.x) low = mid; else high = mid;
     }
     const kvae_adamw_tensor t = g.t[low];
-    const long at = (long)(blockIdx.x - g.first_chunk[low]) * ADAM_CHUNK + (long)threadIdx.x * PER_LANE;
-    const long left = t.numel - at;
-    const int n = left >= PER_LANE ? PER_LANE : (left > 0 ? (int)left : 0);
-    const long block = at / QUANT_BLOCK;
+    const long block = (long)(blockIdx.x - g.first_chunk[low]) * (ADAM_CHUNK / QUANT_BLOCK) + threadIdx.x / 16;
+    const int inside = (threadIdx.x & 15) * GROUP;
+    const long at = block * QUANT_BLOCK + inside, n = t.numel - at;
     // a row of 16 lanes (one block) leaves together, so that max16 finds all its lanes
     if (block * QUANT_BLOCK >= t.numel) return;
-    float p[PER_LANE], grad[PER_LANE], m[PER_LANE], v[PER_LANE];
-    if constexpr (MASTER) {
-        load16<float>(static_cast<const float*>(t.master) + at, n, p);
-    } else {
-        load16<T>(static_cast<const T*>(t.param) + at, n, p);
-    }
-    load16<T>(static_cast<const T*>(t.grad) + at, n, grad);
-    if constexpr (EIGHT) {
-        load_codes(static_cast<const uint8_t*>(t.exp_avg) + at, n,
-                   static_cast<const float*>(t.exp_avg_scale)[block], m);
-        load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at, n,
-                   static_cast<const float*>(t.exp_avg_sq_scale)[block], v);
+    const auto update = [&](auto full) {
+#pragma clang fp contract(off)
+        constexpr bool FULL = decltype(full)::value;
+        float p[PER_LANE], grad[PER_LANE], m[PER_LANE], v[PER_LANE];
+        if constexpr (MASTER) {
+            load16<FULL>(static_cast<const float*>(t.master) + at, n, p);
+        } else {
+            load16<FULL>(static_cast<const T*>(t.param) + at, n, p);
+        }
+        load16<FULL>(static_cast<const T*>(t.grad) + at, n, grad);
+        if constexpr (EIGHT) {
+            load_codes<FULL>(static_cast<const uint8_t*>(t.exp_avg) + at, n,
+                             static_cast<const float*>(t.exp_avg_scale)[block], m);
+            load_codes<FULL>(static_cast<const uint8_t*>(t.exp_avg_sq) + at, n,
+                             static_cast<const float*>(t.exp_avg_sq_scale)[block], v);
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) v[i] = v[i] * v[i];
-    } else {
-        load16<float>(static_cast<const float*>(t.exp_avg) + at, n, m);
-        load16<float>(static_cast<const float*>(t.exp_avg_sq) + at, n, v);
-    }
+            for (int i = 0; i < PER_LANE; ++i) v[i] = v[i] * v[i];
+        } else {
+            load16<FULL>(static_cast<const float*>(t.exp_avg) + at, n, m);
+            load16<FULL>(static_cast<const float*>(t.exp_avg_sq) + at, n, v);
+        }
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-        m[i] = m[i] * g.beta1 + grad[i] * g.one_minus_beta1;
-        v[i] = v[i] * g.beta2 + (grad[i] * grad[i]) * g.one_minus_beta2;
-        const float root = sqrtf(v[i]);
-        if constexpr (EIGHT) v[i] = root;            // from here on sqrt(v)
-        p[i] = p[i] * (1.f - decay) - rate * (m[i] / (root * root_fix + g.eps));
-    }
-    if constexpr (MASTER) store16<float>(static_cast<float*>(t.master) + at, n, p);
-    store16<T>(static_cast<T*>(t.param) + at, n, p);
-    if constexpr (EIGHT) {
-        const bool first = at == block * QUANT_BLOCK;
-        const unsigned index = g.first_block[low] * (unsigned)QUANT_BLOCK + (unsigned)at;
-        store_codes<false, 0>(static_cast<uint8_t*>(t.exp_avg) + at,
-                              static_cast<float*>(t.exp_avg_scale) + block, first, n, m, index, key);
-        store_codes<true, 1>(static_cast<uint8_t*>(t.exp_avg_sq) + at,
-                             static_cast<float*>(t.exp_avg_sq_scale) + block, first, n, v, index, key);
+        for (int i = 0; i < PER_LANE; ++i) {
+            m[i] = m[i] * g.beta1 + grad[i] * g.one_minus_beta1;
+            v[i] = v[i] * g.beta2 + (grad[i] * grad[i]) * g.one_minus_beta2;
+            const float root = sqrtf(v[i]);
+            if constexpr (EIGHT) v[i] = root;        // from here on sqrt(v)
+            // (the reciprocal is within an ulp; a quotient to the last bit would cost eight
+            // instructions and moves the update by 1e-7 of itself)
+            p[i] = p[i] * (1.f - decay) - rate * (m[i] * __builtin_amdgcn_rcpf(root * root_fix + g.eps));
+        }
+        if constexpr (MASTER) store16<FULL>(static_cast<float*>(t.master) + at, n, p);
+        store16<FULL>(static_cast<T*>(t.param) + at, n, p);
+        if constexpr (EIGHT) {
+            const bool first = inside == 0;
+            const unsigned index = g.first_block[low] * (unsigned)QUANT_BLOCK + (unsigned)at;
+            const unsigned h = index * INDEX_FACTOR + key;
+            unsigned random[PER_LANE];
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i)
+                random[i] = random_bits(h + (unsigned)((i / GROUP) * APART + i % GROUP) * INDEX_FACTOR);
+            store_codes<FULL, false, 0>(static_cast<uint8_t*>(t.exp_avg) + at,
+                                        static_cast<float*>(t.exp_avg_scale) + block, first, n, m, random);
+            store_codes<FULL, true, 1>(static_cast<uint8_t*>(t.exp_avg_sq) + at,
+                                       static_cast<float*>(t.exp_avg_sq_scale) + block, first, n, v, random);
+        } else {
+            store16<FULL>(static_cast<float*>(t.exp_avg) + at, n, m);
+            store16<FULL>(static_cast<float*>(t.exp_avg_sq) + at, n, v);
+        }
+    };
+    if ((long)(blockIdx.x - g.first_chunk[low] + 1) * ADAM_CHUNK <= t.numel) {
+        update(std::true_type{});
     } else {
-        store16<float>(static_cast<float*>(t.exp_avg) + at, n, m);
-        store16<float>(static_cast<float*>(t.exp_avg_sq) + at, n, v);
+        update(std::false_type{});
     }
 }
 
