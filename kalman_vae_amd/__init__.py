@@ -6,7 +6,7 @@ Compute runs only in the HIP library kalman_vae_amd/csrc/libkvae_kalman.so
 """
 from .sample_control import SampleControl
 from .misc import aggregate
-from .dynamics_parameter_network import LSTMModel, MLPModel
+from .dynamics_parameter_network import GatedModel, LSTMModel, MLPModel
 from .state_space_model import StateSpaceModel
 from .elbo import kalman_elbo
 from .variational_autoencoder import BernoulliDecoder, Encoder, GaussianDecoder
@@ -17,7 +17,8 @@ from .optim import AdamW, adamw_step
 from .functions import (kalman_filter_steps, kalman_smooth_steps, kalman_elbo_terms,
                         read_status)
 
-__all__ = ["SampleControl", "aggregate", "LSTMModel", "MLPModel", "StateSpaceModel",
+__all__ = ["SampleControl", "aggregate", "GatedModel", "LSTMModel", "MLPModel",
+           "StateSpaceModel",
            "kalman_elbo", "KalmanVariationalAutoencoder", "Encoder", "GaussianDecoder",
            "BernoulliDecoder", "kalman_filter_steps", "kalman_smooth_steps", "kalman_elbo_terms",
            "read_status", "gated_scan", "gated_scan_step", "rms_norm",

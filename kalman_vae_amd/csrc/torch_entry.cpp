@@ -91,6 +91,12 @@ Tensor rows_dense(const Tensor& t) {
 // (rows, D) with last-axis stride 1; copies only when the leading axes do not merge
 Tensor as_rows(const Tensor& t, int64_t D) { return rows_dense(t).reshape({-1, D}); }
 
+// A tensor that a kernel has written in place: autograd's saved copies of it are stale, and whoever
+// keeps something made from it can see so.
+void changed(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Gradients of a gradient are refused when they are asked for, not when the graph is built.
 variable_list once_differentiable(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -180,6 +186,7 @@ Tensor gated_scan_step(const Tensor& u_in, const Tensor& state, const OptTensor&
     Tensor y = empty({B, H}, u);
     check(lib.scan_step(B, H, dtype_code(u.scalar_type()), gated, u.data_ptr(), u.stride(0), address(mask),
                         mask ? mask->stride(0) : 0, state.data_ptr(), y.data_ptr(), on.stream));
+    changed(state);
     return y;
 }
 
@@ -414,6 +421,9 @@ void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::
                             pairs ? ms[i]->data_ptr() : nullptr, pairs ? vs[i]->data_ptr() : nullptr,
                             masters.empty() ? nullptr : masters[i]->data_ptr()};
         blocks += (n + KVAE_ADAMW_BLOCK - 1) / KVAE_ADAMW_BLOCK;
+        for (const Tensor* t : {params[i], m[i], v[i], pairs ? ms[i] : m[i], pairs ? vs[i] : v[i],
+                                masters.empty() ? m[i] : masters[i]})
+            changed(*t);
         if (d.count == KVAE_ADAMW_MAX_TENSORS) launch();
     }
     if (d.count) launch();

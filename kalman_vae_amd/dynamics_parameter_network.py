@@ -1,4 +1,5 @@
-"""Dynamics-parameter ("weight") networks: (t,B,a_dim) -> softmax (t,B,K).
+"""Dynamics-parameter ("weight") networks: (t,B,a_dim) -> softmax (t,B,K): the reference's
+LSTM and perceptron, and a stack of gated linear recurrences.
 
 Ordinary PyTorch modules whose hot parts run on the package's HIP kernels when
 the tensors are float32 on a GPU (LSTM recurrence for whole-sequence calls, the
@@ -9,7 +10,10 @@ reference (kvae/dynamics_parameter_network.py:18-90) so its checkpoints load:
 import torch
 import torch.nn as nn
 
+from . import _capi as capi
 from . import lstm_function
+from .sequence_ops import (gated_scan, gated_scan_step, linear_8bit, quantize_rows, rms_norm,
+                           rms_norm_quantized)
 
 
 class LSTMModel(nn.Module):
@@ -138,9 +142,206 @@ class MLPModel(nn.Module):
     is_recurrent = False
 
 
+def _plain_norm(x, weight, eps):
+    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * weight
+
+
+def _plain_scan(u, state):
+    """gated_scan by its definition, one step after the other (CPU and float64)."""
+    x, forget, gate = u.chunk(3, dim=-1)
+    f, keep = torch.sigmoid(forget), torch.sigmoid(-forget)
+    c = torch.zeros_like(x[0]) if state is None else state
+    steps = []
+    for t in range(u.shape[0]):
+        c = f[t] * c + keep[t] * x[t]
+        steps.append(c)
+    return torch.stack(steps) * torch.nn.functional.silu(gate), c
+
+
+class GatedBlock(nn.Module):
+    """norm -> projection to [x | forget | gate] -> gated recurrence -> projection back."""
+
+    def __init__(self, hidden_dim):
+        super().__init__()
+        self.norm = nn.Parameter(torch.ones(hidden_dim))
+        self.proj = nn.Linear(hidden_dim, 3 * hidden_dim)
+        self.out = nn.Linear(hidden_dim, hidden_dim)
+        with torch.no_grad():                  # gates that mostly remember to begin with
+            self.proj.bias[hidden_dim:2 * hidden_dim] += 1.0
+
+
+class GatedModel(nn.Module):
+    """A stack of gated linear recurrences with pre-norm residuals:
+
+        h = embed(x);  per block: h += out(scan(proj(norm(h))));  weights = softmax(linear(norm(h)))
+
+    The recurrent alternative to ``LSTMModel`` whose time axis holds no matrix product: all
+    projections run over the whole sequence at once and the recurrence between them is a scan
+    (``gated_scan``), which also runs parallel in time.  Used like the LSTM: the state is cached on
+    the module between calls, and feeding a sequence one step at a time equals feeding it whole.
+    On a GPU in float32, bfloat16 or float16 the norms and scans are the package's HIP kernels; on the
+    CPU and in float64 the module is plain torch.
+
+    ``eight_bit()`` lays the blocks' projection weights out in 8 bits; calls that record no gradient
+    then run the projections as ``linear_8bit`` on the norm's 8-bit output.  The reference has no
+    counterpart of this network (kvae/dynamics_parameter_network.py:18-90 has the LSTM and the MLP)."""
+
+    eps = 1e-6
+    is_recurrent = True
+
+    def __init__(self, input_dim, output_dim, hidden_dim, num_layers):
+        super().__init__()
+        if num_layers < 1:
+            raise ValueError(f"num_layers must be at least 1, got {num_layers}")
+        self.hidden_dim = hidden_dim
+        self.num_layers = num_layers
+        self.embed = nn.Linear(input_dim, hidden_dim)
+        self.blocks = nn.ModuleList(GatedBlock(hidden_dim) for _ in range(num_layers))
+        self.norm = nn.Parameter(torch.ones(hidden_dim))
+        self.linear = nn.Linear(hidden_dim, output_dim)
+        self.use_hip_kernels = True
+        self._states = None                    # one (B,H) per block, or None
+        self._eight = None                     # see eight_bit()
+        self.count = 0
+
+    # -- state carried between calls --------------------------------------------------------
+    @property
+    def hidden(self):
+        """The state carried between calls, (num_layers, B, hidden_dim), or None."""
+        return None if self._states is None else torch.stack(self._states)
+
+    @hidden.setter
+    def hidden(self, value):
+        self._states = None if value is None else list(value.unbind(0))
+
+    def clear_hidden_state(self):
+        self._states = None
+        self.count = 0
+
+    def reset_hidden_state(self, batch_size, device, dtype):
+        self.hidden = torch.zeros(self.num_layers, batch_size, self.hidden_dim, device=device,
+                                  dtype=torch.float32 if dtype in capi.SEQUENCE_DTYPES else dtype)
+        self.count = 0
+
+    # -- 8-bit serving form -----------------------------------------------------------------
+    def eight_bit(self, on=True):
+        """Lay out (or, with ``on=False``, drop) the 8-bit form of the blocks' projections: 1 byte per
+        weight and one float32 scale per output.  Later calls without a gradient use it; a call
+        after the parameters have changed raises until this is called again.  Returns self."""
+        self._eight = None
+        if on:
+            capi.require_gpu(self.norm)
+            with torch.no_grad():
+                self._eight = [tuple(quantize_rows(layer.weight) + (layer.bias.float(), layer.weight._version,
+                                                                    layer.bias._version)
+                                     for layer in (block.proj, block.out)) for block in self.blocks]
+        return self
+
+    def _apply(self, fn):
+        self._eight = None                     # moved or converted parameters
+        return super()._apply(fn)
+
+    def _product_8bit(self, i, which, q, scale, dtype):
+        weight, weight_scale, bias, *versions = self._eight[i][which]
+        layer = (self.blocks[i].proj, self.blocks[i].out)[which]
+        if versions != [layer.weight._version, layer.bias._version]:
+            raise RuntimeError("the parameters have changed since eight_bit(): call it again")
+        return linear_8bit(q, scale, weight, weight_scale, bias=bias, dtype=dtype)
+
+    # -- forward ----------------------------------------------------------------------------
+    def _on_kernels(self, x):
+        return (self.use_hip_kernels and x.is_cuda and x.dtype in capi.SEQUENCE_DTYPES
+                and self.hidden_dim <= capi.NORM_MAX_WIDTH)
+
+    def _stack(self, x, scan):
+        """(branch, h) behind the last block; scan(i, u) runs block i's recurrence."""
+        kernels = self._on_kernels(x)
+        eight = kernels and self._eight is not None and not torch.is_grad_enabled()
+        h, branch = lstm_function.linear(x, self.embed), None
+        for i, block in enumerate(self.blocks):
+            if eight:
+                if branch is None:
+                    q, scale = rms_norm_quantized(h, block.norm, eps=self.eps)
+                else:
+                    q, scale, h = rms_norm_quantized(branch, block.norm, residual=h, eps=self.eps)
+                # (bfloat16 between the products: its rounding is far below that of 8 bits)
+                y = scan(i, self._product_8bit(i, 0, q, scale, torch.bfloat16))
+                branch = self._product_8bit(i, 1, *quantize_rows(y), x.dtype)
+            else:
+                n, h = self._norm(h, branch, block.norm, kernels)
+                branch = lstm_function.linear(scan(i, lstm_function.linear(n, block.proj)), block.out)
+        return self._norm(h, branch, self.norm, kernels)[0]
+
+    def _norm(self, h, branch, weight, kernels):
+        """(norm of h + branch, h + branch)"""
+        if not kernels:
+            h = h if branch is None else h + branch
+            return _plain_norm(h, weight, self.eps), h
+        if branch is None:
+            return rms_norm(h, weight, eps=self.eps), h
+        return rms_norm(branch, weight, residual=h, eps=self.eps)
+
+    def forward(self, x, lead=False):
+        """x (t,B,a_dim) -> weights (t,B,K); lead=True prepends the uniform weights
+        of the step before the first observation: (t+1,B,K)."""
+        self.count += 1
+        kernels = self._on_kernels(x)
+        states, ends = self._states, []
+        fresh = states is None and x.size(0) > 1
+
+        def scan(i, u):
+            first = None if states is None else states[i]
+            y, end = gated_scan(u, first) if kernels else _plain_scan(u, first)
+            # (as in LSTMModel: a whole sequence from a fresh state leaves a state without a graph)
+            ends.append(end.detach() if fresh else end)
+            return y
+
+        n = self._stack(x, scan)
+        self._states = ends
+        return lstm_function.softmax_head(n, self.linear, lead)
+
+    def inference_stepper(self, x):
+        """For a caller that feeds one step at a time without a gradient (the masked filter): an
+        object whose ``step(x_t (B,a_dim), out (B,K))`` equals ``out.copy_(self(x_t[None])[0])`` with
+        the state updated in place (``gated_scan_step``), or None when that form does not apply.
+        Call ``finish_steps`` afterwards so that the module carries the state on."""
+        if (torch.is_grad_enabled() or x.dim() != 2 or x.dtype != torch.float32 or not self._on_kernels(x)
+                or not lstm_function.head_supported(x.new_empty(1, self.hidden_dim), self.linear)):
+            return None
+        return GatedStepper(self, x)
+
+    def finish_steps(self, stepper, steps):
+        self._states = stepper.states
+        self.count += steps
+
+
+class GatedStepper:
+    """See ``GatedModel.inference_stepper``."""
+
+    def __init__(self, model, x):
+        self.model, B = model, x.shape[0]
+        self.states = [torch.zeros(B, model.hidden_dim, device=x.device) if model._states is None
+                       else model._states[i].clone() for i in range(model.num_layers)]
+
+    @torch.no_grad()
+    def step(self, x, out):
+        """x (B,P) -> out (B,K), contiguous float32; advances the carried state."""
+        model = self.model
+        if not (out.is_contiguous() and out.shape == (x.shape[0], model.linear.out_features)
+                and x.dtype == out.dtype == torch.float32):
+            raise ValueError("GatedStepper.step: x (B,P) and contiguous out (B,K) must be float32")
+        n = model._stack(x, lambda i, u: gated_scan_step(u, self.states[i]))
+        W, b = model.linear.weight.contiguous(), model.linear.bias.contiguous()
+        capi.check(capi.load().kvae_softmax_head_forward(
+            n.shape[0], model.hidden_dim, W.shape[0], n.data_ptr(), W.data_ptr(), b.data_ptr(),
+            out.data_ptr(), 0, capi.current_stream_ptr()))
+
+
 def make_weight_model(kind, a_dim, K, hidden_dim, num_layers):
     if kind == "mlp":
         return MLPModel(a_dim, K, hidden_dim=hidden_dim, num_layers=num_layers)
     if kind == "lstm":
         return LSTMModel(a_dim, K, hidden_dim=hidden_dim, num_layers=num_layers)
+    if kind == "gated":
+        return GatedModel(a_dim, K, hidden_dim=hidden_dim, num_layers=num_layers)
     raise ValueError("Invalid dynamics_parameter_network: {}".format(kind))
