@@ -36,19 +36,30 @@ struct LinearArgs {
     void* y;
 };
 
-// 16 bytes of a row from byte k on; bytes at K and beyond, and rows that are not there, are zero.
-__device__ __forceinline__ v4i load_chunk(const uint8_t* row, bool there, int k, int K) {
-    v4i r = {0, 0, 0, 0};
-    if (there && k + 16 <= K) {
-        struct __attribute__((packed)) Any { v4i v; };
-        r = reinterpret_cast<const Any*>(row + k)->v;
-    } else if (there && k < K) {
-        for (int i = 0; k + i < K; ++i) {
-            const int b = (int)row[k + i] << (8 * (i & 3));
-            if (i < 4) r.x |= b; else if (i < 8) r.y |= b; else if (i < 12) r.z |= b; else r.w |= b;
-        }
+struct __attribute__((packed)) AnyPiece { v4i v; };
+
+// 16 bytes of a row of K from byte k on, at any address; bytes at K and beyond are zero.  A piece that
+// ends behind the row is the row's last 16 bytes shifted down.
+__device__ __forceinline__ v4i load_piece(const uint8_t* row, int k, int K) {
+    if (k + 16 <= K) return reinterpret_cast<const AnyPiece*>(row + k)->v;
+    unsigned long lo = 0, hi = 0;
+    if (k >= K) {
+    } else if (K >= 16) {
+        const v4i r = reinterpret_cast<const AnyPiece*>(row + K - 16)->v;
+        lo = (unsigned)r.x | (unsigned long)(unsigned)r.y << 32;
+        hi = (unsigned)r.z | (unsigned long)(unsigned)r.w << 32;
+        const int shift = 8 * (k + 16 - K);          // 8 .. 120
+        lo = shift < 64 ? lo >> shift | hi << (64 - shift) : hi >> (shift - 64);
+        hi = shift < 64 ? hi >> shift : 0;
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < K; ++i) (i < 8 ? lo : hi) |= (unsigned long)row[i] << (8 * (i & 7));
     }
-    return r;
+    return v4i{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+}
+// the same, or zero where there is no such row
+__device__ __forceinline__ v4i load_chunk(const uint8_t* row, bool there, int k, int K) {
+    return load_piece(row, there ? k : K, K);
 }
 
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -230,6 +241,167 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(LinearArgs g) {
             }
 }
 
+// Large products: 256 x 256 tiles, four wavefronts of 128 x 128 each (their sums fill the accumulation
+// registers, one wavefront per SIMD).  A 64-byte slice of k is sixteen 32x32x64 matrix instructions
+// (1024 cycles) per wavefront on eight operands of 2 KB, so that the four wavefronts ask LDS for 64 bytes
+// a cycle, half of what 64 x 64 wavefront tiles would.
+//
+// Slices go from memory straight into LDS (no registers in between), into four buffers in turn: while
+// slice s is multiplied, the operands of s + 1 are read into registers of their own and s + 2 and s + 3 are
+// on their way.  One barrier per slice: a wavefront waits until its own pieces of s + 1 have arrived, and
+// behind the barrier everybody's have; the buffer that s + 3 goes to held s - 1, whose operands everybody
+// had read before.
+//
+// Rows that are not there repeat the last one (their results are not stored).  Where k ends inside the
+// last slice, pieces behind the end repeat the row's last piece and are replaced by zero on their way
+// from LDS to the registers, in both operands (a NaN in one of them must not meet the other's zero).
+constexpr int BIG = 256, BIG_SLICE = 64, BUFFERS = 4;
+constexpr int OPERAND = BIG * BIG_SLICE / 16;        // pieces of one operand's slice
+
+template <typename T>
+__global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int tiles_n, int tiles_m) {
+    __shared__ v4i lds[BUFFERS * 2 * OPERAND];       // [buffer][x, w][row][4 pieces, see below]: 128 KB
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Workgroups go round the eight dies (blockIdx % 8): each die gets a run of neighbouring tiles, in
+    // groups of eight rows of tiles, so that its cache serves the tiles that run together.
+    const int total = tiles_n * tiles_m, per = (total + 7) / 8;
+    const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int in_group = 8 * tiles_n, group = id / in_group, rest = id - group * in_group;
+    const int rows = tiles_m - 8 * group < 8 ? tiles_m - 8 * group : 8;
+    const long m0 = (long)(8 * group + rest % rows) * BIG;
+    const int n0 = rest / rows * BIG;
+    const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
+
+    // Piece c of row r lies at place c ^ (r / 4 % 4) of the row, which spreads a column of pieces over
+    // the banks.  An instruction moves 16 rows: lane l fills place l % 4 of row l / 4.
+    const int piece = (lane & 3) ^ ((lane >> 4) & 3), last_piece = g.K / 16 - 1;
+    const uint8_t* xb = g.x + m0 * g.K;
+    const uint8_t* wb = g.w + (long)n0 * g.K;
+    const long rows_x = g.M - m0, rows_w = g.N - n0;
+    unsigned x_row[4], w_row[4];                     // byte offsets of the lane's rows
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long r = 16 * (wave + 4 * i) + (lane >> 2);
+        x_row[i] = (unsigned)(r < rows_x ? r : rows_x - 1) * (unsigned)g.K;
+        w_row[i] = (unsigned)(r < rows_w ? r : rows_w - 1) * (unsigned)g.K;
+    }
+    const auto fetch = [&](int s) {
+        const int p = 4 * s + piece;
+        const unsigned k = 16u * (unsigned)(p < last_piece ? p : last_piece);
+        v4i* at = lds + (s % BUFFERS) * 2 * OPERAND + wave * 64;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(xb + (x_row[i] + k)),
+                (__attribute__((address_space(3))) void*)(at + 256 * i), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(wb + (w_row[i] + k)),
+                (__attribute__((address_space(3))) void*)(at + OPERAND + 256 * i), 16, 0, 0);
+        }
+    };
+    struct Operands {
+        v8i a[4], b[4];
+    };
+    const int turn = (lane >> 5) * 2 ^ ((lane >> 2) & 3), row4 = (lane & 31) * 4;
+    const auto read = [&](int s, Operands& h) {
+        const v4i* x = lds + (s % BUFFERS) * 2 * OPERAND + wm * 4 + row4;
+        const v4i* w = lds + (s % BUFFERS) * 2 * OPERAND + OPERAND + wn * 4 + row4;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const v4i p = w[128 * t + turn], q = w[128 * t + (turn ^ 1)];
+            h.a[t] = v8i{p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+            const v4i u = x[128 * t + turn], v = x[128 * t + (turn ^ 1)];
+            h.b[t] = v8i{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        }
+    };
+    v16f acc[4][4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+    const auto multiply = [&](const Operands& h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(h.a[i], h.b[j], acc[i][j], 0, 0, 0,
+                                                                            0, 0, 0);
+    };
+    // Multiplies slice s from `now` and reads slice s + 1 into `next`.  The eight pieces that a wavefront
+    // asks for last (slice s + 2) may still be on their way, those of s + 1 may not, and its own reads of
+    // slice s are done (they were issued half a step ago or earlier).  The reads go between the first
+    // eight matrix instructions, the requests between the others.
+    const auto step = [&](int s, const Operands& now, Operands& next) {
+        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(s + 1, next);
+        fetch(s + 3);
+        multiply(now);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a matrix instruction
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // two reads
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);   // a request
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // zero where slice s is behind the end of k
+    const auto cut = [&](int s, Operands& h) {
+        const int there = g.K / 16 - 4 * s - (lane >> 5) * 2;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                h.a[t][i] = there > i / 4 ? h.a[t][i] : 0;
+                h.b[t][i] = there > i / 4 ? h.b[t][i] : 0;
+            }
+    };
+    // Slices are walked in pairs (one of zeros is added to an odd number), so that the loop is one
+    // straight run; what it fetches behind the end is not used.
+    const int pairs = (g.K + 2 * BIG_SLICE - 1) / (2 * BIG_SLICE);
+    fetch(0);
+    fetch(1);
+    fetch(2);
+    Operands even, odd;
+    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, even);
+    for (int p = 0; p < pairs - 1; ++p) {
+        step(2 * p, even, odd);
+        step(2 * p + 1, odd, even);
+    }
+    const int s = 2 * (pairs - 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (nothing may still be written when others take over the LDS)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(s + 1, odd);
+    cut(s, even);
+    multiply(even);
+    cut(s + 1, odd);
+    multiply(odd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                                    acc[i][j][4 * q + 3]};
+                store4<T>(g, m0 + wm + 32 * j + (lane & 31), n0 + wn + 32 * i + 8 * q + 4 * (lane >> 5), v);
+            }
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 }  // namespace kvae
 
 using namespace kvae;
@@ -253,6 +425,12 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
                 linear_few_rows_kernel<T, 2><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
             } else {
                 linear_few_rows_kernel<T, 4><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
+            }
+        } else if (!WIDENED<T> && K % 16 == 0 && K < (1 << 22) && aligned16(x) && aligned16(w) && ((M + BIG - 1) / BIG) * ((N + BIG - 1) / BIG) >= 128) {
+            if constexpr (!WIDENED<T>) {
+                const long tn = (N + BIG - 1) / BIG, tm = (M + BIG - 1) / BIG;
+                const unsigned blocks = (unsigned)((tn * tm + 7) / 8 * 8);
+                linear_big_kernel<T><<<dim3(blocks), 256, 0, s>>>(g, (int)tn, (int)tm);
             }
         } else {
             const long my = (M + TILE - 1) / TILE;

@@ -86,6 +86,27 @@ def test_whole_numbers_are_exact():
         assert torch.equal(y.double(), a.double() @ b.double().t().contiguous())
 
 
+@pytest.mark.parametrize("M,N,K", [(2816, 2816, 16), (2817, 2900, 48), (4096, 2048, 64), (3000, 3000, 128), (2600, 3333, 176),
+                                   (5000, 1793, 208), (2304, 3328, 1040)])
+def test_large_tiles(M, N, K):
+    """Enough 256 x 256 tiles for the large form, ragged in rows, columns and k; NaN behind the rows."""
+    import kalman_vae_amd as kv
+    x, sx, w, sw, bias = make(M, N, K, seed=K)
+    pads = []
+    for t in (x, w):
+        buf = torch.full((t.numel() + 65536,), 0x7F, dtype=torch.uint8, device="cuda")
+        buf[:t.numel()].copy_(t.reshape(-1).view(torch.uint8))
+        pads.append(buf[:t.numel()].view(torch.float8_e4m3fn).view(t.shape))
+    y = kv.linear_8bit(pads[0], sx, pads[1], sw, bias=bias, dtype=torch.float16)
+    rows = torch.cat([torch.arange(0, M, 37), torch.arange(M - 3, M)]).cuda()
+    check(y[rows], x[rows], sx[rows], w, sw, bias)
+    # whole numbers of few bits: exact sums (below 2048 and in steps of one)
+    a, b = (torch.randint(-1, 2, t.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(7)) for t in (x, w))
+    one = lambda n: torch.ones(n, device="cuda")  # noqa: E731
+    y = kv.linear_8bit(a.float().to(torch.float8_e4m3fn), one(M), b.float().to(torch.float8_e4m3fn), one(N), dtype=torch.float16)
+    assert torch.equal(y.float(), a.float() @ b.float().t().contiguous())
+
+
 def test_layouts():
     """Leading axes, rows at odd addresses, a transposed weight, a broadcast row."""
     import kalman_vae_amd as kv
