@@ -38,23 +38,26 @@ struct LinearArgs {
 
 struct __attribute__((packed)) AnyPiece { v4i v; };
 
+// r without its first `bytes` (0 .. 16 and more), zero behind what is left
+__device__ __forceinline__ v4i shift_down(const v4i& r, int bytes) {
+    unsigned long lo = (unsigned)r.x | (unsigned long)(unsigned)r.y << 32;
+    unsigned long hi = (unsigned)r.z | (unsigned long)(unsigned)r.w << 32;
+    const int n = 8 * (bytes & 7);
+    if (bytes >= 8) lo = hi, hi = 0;
+    if (n) lo = lo >> n | hi << (64 - n), hi >>= n;
+    if (bytes >= 16) lo = 0;
+    return v4i{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+}
+
 // 16 bytes of a row of K from byte k on, at any address; bytes at K and beyond are zero.  A piece that
 // ends behind the row is the row's last 16 bytes shifted down.
 __device__ __forceinline__ v4i load_piece(const uint8_t* row, int k, int K) {
     if (k + 16 <= K) return reinterpret_cast<const AnyPiece*>(row + k)->v;
+    if (k >= K) return v4i{0, 0, 0, 0};
+    if (K >= 16) return shift_down(reinterpret_cast<const AnyPiece*>(row + K - 16)->v, k + 16 - K);
     unsigned long lo = 0, hi = 0;
-    if (k >= K) {
-    } else if (K >= 16) {
-        const v4i r = reinterpret_cast<const AnyPiece*>(row + K - 16)->v;
-        lo = (unsigned)r.x | (unsigned long)(unsigned)r.y << 32;
-        hi = (unsigned)r.z | (unsigned long)(unsigned)r.w << 32;
-        const int shift = 8 * (k + 16 - K);          // 8 .. 120
-        lo = shift < 64 ? lo >> shift | hi << (64 - shift) : hi >> (shift - 64);
-        hi = shift < 64 ? hi >> shift : 0;
-    } else {
 #pragma unroll 1
-        for (int i = 0; i < K; ++i) (i < 8 ? lo : hi) |= (unsigned long)row[i] << (8 * (i & 7));
-    }
+    for (int i = 0; k + i < K; ++i) (i < 8 ? lo : hi) |= (unsigned long)row[k + i] << (8 * (i & 7));
     return v4i{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 // the same, or zero where there is no such row
@@ -97,6 +100,65 @@ __device__ __forceinline__ void store4(const LinearArgs& g, long m, int n, const
         for (int i = 0; i < 4; ++i)
             if (n + i < g.N) out[i] = narrow<T>(acc[i] * sx * g.sw[n + i] + (g.bias ? g.bias[n + i] : 0.f));
     }
+}
+
+// Results of 32 rows by WN columns that a wavefront holds as WN / 32 sums of a 32 x 32 instruction:
+// a lane has row lane % 32, columns 32 i + 8 q + 4 (lane / 32) .. + 3.  Written from there, an
+// instruction would touch 32 rows with 16 bytes each; they go through LDS (`region`: the wavefront's own,
+// 32 rows) and out in runs of a whole row of WN.  value(i, e): element e of sum i.
+template <typename T, int WN, typename F>
+__device__ __forceinline__ void write_rows(const LinearArgs& g, char* region, long m0, int n0, int lane, F&& value) {
+    constexpr int ROW = WN * (int)sizeof(T), CHUNKS = ROW / 16, PER = 16 / (int)sizeof(T);
+    const int row = lane & 31;
+    const long last = g.M - 1;
+    const float sx = g.sx[m0 + row < last ? m0 + row : last];
+#pragma unroll
+    for (int i = 0; i < WN / 32; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int in = 32 * i + 8 * q + 4 * (lane >> 5), n = n0 + in;
+            Pack<float, 4> sw{}, b{};
+            if (n + 4 <= g.N) {
+                sw = load_pack<float, 4>(g.sw + n);
+                if (g.bias) b = load_pack<float, 4>(g.bias + n);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < g.N) {
+                        sw.v[e] = g.sw[n + e];
+                        if (g.bias) b.v[e] = g.bias[n + e];
+                    }
+            }
+            Pack<T, 4> p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p.v[e] = narrow<T>(value(i, 4 * q + e) * sx * sw.v[e] + b.v[e]);
+            // (the exclusive-or spreads the rows over the banks)
+            const int chunk = in / PER ^ (row & (CHUNKS - 1));
+            *reinterpret_cast<Pack<T, 4>*>(region + row * ROW + chunk * 16 + in % PER * (int)sizeof(T)) = p;
+        }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    constexpr int ROWS = 64 / CHUNKS;                // rows of one instruction
+    T* y = static_cast<T*>(g.y);
+#pragma unroll
+    for (int k = 0; k < 32 / ROWS; ++k) {
+        const int r = k * ROWS + lane / CHUNKS, c = lane % CHUNKS, n = n0 + c * PER;
+        const Pack<T, PER> p = *reinterpret_cast<const Pack<T, PER>*>(region + r * ROW + (c ^ (r & (CHUNKS - 1))) * 16);
+        if (m0 + r < g.M) {
+            T* out = y + (m0 + r) * g.N + n;
+            if (n + PER <= g.N) {
+                store_pack<T, PER>(out, p);
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; ++e)
+                    if (n + e < g.N) out[e] = p.v[e];
+            }
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 constexpr int FEW_WAVES = 8;
@@ -162,8 +224,9 @@ constexpr int TILE = 128, SLICE = 128;
 __device__ __forceinline__ int piece_at(int r, int c) { return r * (SLICE / 16) + (c ^ (r & 7)); }
 
 template <typename T>
-__global__ void __launch_bounds__(256) linear_tile_kernel(LinearArgs g) {
-    __shared__ v4i xs[TILE * SLICE / 16], ws[TILE * SLICE / 16];
+__global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
+    __shared__ v4i shared[2 * TILE * SLICE / 16];
+    v4i *xs = shared, *ws = shared + TILE * SLICE / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long m0 = (long)blockIdx.y * TILE;
     const int n0 = blockIdx.x * TILE;
@@ -175,25 +238,19 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(LinearArgs g) {
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
-    v4i xr[4], wr[4];
-    const auto fetch = [&](int k0) {
+    // A thread's pieces: column tid % 8 of rows tid / 8 + 32 i, as 32-bit offsets from the tile's first
+    // rows; rows that are not there repeat the last (their results are not stored).
+    const uint8_t* xb = g.x + m0 * g.K;
+    const uint8_t* wb = g.w + (long)n0 * g.K;
+    const int col = (threadIdx.x & 7) * 16;
+    unsigned x_row[4], w_row[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int q = threadIdx.x + 256 * i, r = q >> 3, k = k0 + (q & 7) * 16;
-            xr[i] = load_chunk(g.x + (m0 + r) * g.K, m0 + r < g.M, k, g.K);
-            wr[i] = load_chunk(g.w + (long)(n0 + r) * g.K, n0 + r < g.N, k, g.K);
-        }
-    };
-    fetch(0);
-    for (int k0 = 0; k0 < g.K; k0 += SLICE) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int q = threadIdx.x + 256 * i;
-            xs[piece_at(q >> 3, q & 7)] = xr[i];
-            ws[piece_at(q >> 3, q & 7)] = wr[i];
-        }
-        __syncthreads();
-        if (k0 + SLICE < g.K) fetch(k0 + SLICE);
+    for (int i = 0; i < 4; ++i) {
+        const int r = (threadIdx.x >> 3) + 32 * i;
+        x_row[i] = (unsigned)(r < g.M - m0 ? r : (int)(g.M - m0) - 1) * (unsigned)g.K;
+        w_row[i] = (unsigned)(r < g.N - n0 ? r : g.N - n0 - 1) * (unsigned)g.K;
+    }
+    const auto multiply = [&] {
 #pragma unroll
         for (int s = 0; s < SLICE / 64; ++s) {
             v8i a[2], b[2];
@@ -227,18 +284,46 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(LinearArgs g) {
                                                                                     0, 0, 0, 0, 0, 0);
             }
         }
+    };
+    // The next slice is on its way in registers while the present one is multiplied.  Pieces that end
+    // behind the row are its last 16 bytes (K >= 16 here), shifted down before they go to LDS, so that
+    // there is zero behind the end of k in both operands.
+    const int slices = (g.K + SLICE - 1) / SLICE;
+    v4i xr[4], wr[4];
+    const auto fetch = [&](int s) {
+        const int k = s * SLICE + col;
+        const unsigned at = (unsigned)(k < g.K - 16 ? k : g.K - 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            xr[i] = reinterpret_cast<const AnyPiece*>(xb + (x_row[i] + at))->v;
+            wr[i] = reinterpret_cast<const AnyPiece*>(wb + (w_row[i] + at))->v;
+        }
+    };
+    fetch(0);
+    for (int s = 0; s < slices; ++s) {
+        if ((s + 1) * SLICE > g.K) {
+            const int behind = s * SLICE + col + 16 - g.K;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xr[i] = behind > 0 ? shift_down(xr[i], behind) : xr[i];
+                wr[i] = behind > 0 ? shift_down(wr[i], behind) : wr[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int place = piece_at(threadIdx.x >> 3, threadIdx.x & 7) + 32 * i * (SLICE / 16);
+            xs[place] = xr[i];
+            ws[place] = wr[i];
+        }
+        __syncthreads();
+        if (s + 1 < slices) fetch(s + 1);
+        multiply();
         __syncthreads();
     }
+    char* region = reinterpret_cast<char*>(shared) + wave * (32 * 64 * (int)sizeof(T));
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                                    acc[i][j][4 * q + 3]};
-                store4<T>(g, m0 + wm + 32 * j + (lane & 31), n0 + wn + 32 * i + 8 * q + 4 * (lane >> 5), v);
-            }
+    for (int j = 0; j < 2; ++j)
+        write_rows<T, 64>(g, region, m0 + wm + 32 * j, n0 + wn, lane, [&](int i, int e) { return acc[i][j][e]; });
 }
 
 // Large products: 256 x 256 tiles, four wavefronts of 128 x 128 each (their sums fill the accumulation
@@ -388,16 +473,11 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
     multiply(even);
     cut(s + 1, odd);
     multiply(odd);
+    __syncthreads();                                 // the operands' LDS is free
+    char* region = reinterpret_cast<char*>(lds) + wave * (32 * 128 * (int)sizeof(T));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                                    acc[i][j][4 * q + 3]};
-                store4<T>(g, m0 + wm + 32 * j + (lane & 31), n0 + wn + 32 * i + 8 * q + 4 * (lane >> 5), v);
-            }
+    for (int j = 0; j < 4; ++j)
+        write_rows<T, 128>(g, region, m0 + wm + 32 * j, n0 + wn, lane, [&](int i, int e) { return acc[i][j][e]; });
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -410,41 +490,57 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
                                 const void* w, const void* w_scale, const void* bias, int out_dtype,
                                 void* y, void* stream) {
     if (M < 1 || N < 1 || K < 1 || !x || !x_scale || !w || !w_scale || !y) return KVAE_E_BADARG;
-    if (N > (1 << 30) || K > (1 << 30) || M > (1L << 38)) return KVAE_E_TOOLARGE;
+    // 32-bit offsets inside a tile of 256 rows, 31-bit numbers of tiles
+    if (N > (1 << 30) || K > (1 << 22) || M > (1L << 31) || M > (1L << 44) / N) return KVAE_E_TOOLARGE;
     return for_element_type(out_dtype, [&](auto e) {
         using T = decltype(e);
         const LinearArgs g{(long)M, (int)N, (int)K, static_cast<const uint8_t*>(x),
                            static_cast<const uint8_t*>(w), static_cast<const float*>(x_scale),
                            static_cast<const float*>(w_scale), static_cast<const float*>(bias), y};
         const hipStream_t s = static_cast<hipStream_t>(stream);
-        if (M <= 64) {
-            const unsigned nb = (unsigned)((N + 15) / 16);
-            if (M <= 16) {
-                linear_few_rows_kernel<T, 1><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
-            } else if (M <= 32) {
-                linear_few_rows_kernel<T, 2><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
-            } else {
-                linear_few_rows_kernel<T, 4><<<dim3(nb, 1), 64 * FEW_WAVES, 0, s>>>(g);
-            }
-        } else if (!WIDENED<T> && K % 16 == 0 && K < (1 << 22) && aligned16(x) && aligned16(w) && ((M + BIG - 1) / BIG) * ((N + BIG - 1) / BIG) >= 128) {
-            if constexpr (!WIDENED<T>) {
-                const long tn = (N + BIG - 1) / BIG, tm = (M + BIG - 1) / BIG;
-                const unsigned blocks = (unsigned)((tn * tm + 7) / 8 * 8);
-                linear_big_kernel<T><<<dim3(blocks), 256, 0, s>>>(g, (int)tn, (int)tm);
-            }
-        } else {
-            const long my = (M + TILE - 1) / TILE;
-            // (blockIdx.y is 16 bits: rows beyond go in further launches)
-            for (long first = 0; first < my; first += 65535) {
+        const long tn = (N + TILE - 1) / TILE, tm = (M + TILE - 1) / TILE;
+        const long bn = (N + BIG - 1) / BIG, bm = (M + BIG - 1) / BIG;
+        // Which form, by sizes (bfloat16 results, us):
+        // - up to 64 rows, k < 16, or fewer than 64 tiles of 128 x 128 (a quarter of the card's units): few rows.
+        //   512^3 4.1 against 8.3 in tiles, 128 x 4096 x 4096 21 against 34; at 64 tiles (1024^3) 12 each,
+        //   256 x 4096 x 4096 39 against 34.
+        // - half the card's units or more in tiles of 256 x 256, k long enough to hide that such a tile
+        //   neither starts nor ends under another one's work, and rows of whole 16-byte pieces: large tiles.
+        //   16384 x 4096 with k = 4096: 250 against 338 in tiles of 128; k = 1024: 107 against 97.
+        // (blockIdx.y is 16 bits: rows beyond go in further launches)
+        const auto in_parts = [&](long rows_each, auto&& launch) {
+            for (long first = 0; first < M; first += 65535 * rows_each) {
                 LinearArgs h = g;
-                const long count = my - first < 65535 ? my - first : 65535;
-                h.M = g.M - first * TILE;
-                h.x = g.x + first * TILE * K;
-                h.sx = g.sx + first * TILE;
-                h.y = static_cast<T*>(y) + first * TILE * N;
-                linear_tile_kernel<T><<<dim3((unsigned)((N + TILE - 1) / TILE), (unsigned)count), 256, 0, s>>>(h);
+                const long rows = M - first < 65535 * rows_each ? M - first : 65535 * rows_each;
+                h.M = rows;
+                h.x = g.x + first * K;
+                h.sx = g.sx + first;
+                h.y = static_cast<T*>(y) + first * N;
+                launch(h, (unsigned)((rows + rows_each - 1) / rows_each));
+            }
+            return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
+        };
+        if (M <= 64 || K < 16 || tn * tm < 64) {
+            const unsigned nb = (unsigned)((N + 15) / 16);
+            return in_parts(64, [&](const LinearArgs& h, unsigned count) {
+                if (M <= 16) {
+                    linear_few_rows_kernel<T, 1><<<dim3(nb), 64 * FEW_WAVES, 0, s>>>(h);
+                } else if (M <= 32) {
+                    linear_few_rows_kernel<T, 2><<<dim3(nb), 64 * FEW_WAVES, 0, s>>>(h);
+                } else {
+                    linear_few_rows_kernel<T, 4><<<dim3(nb, count), 64 * FEW_WAVES, 0, s>>>(h);
+                }
+            });
+        }
+        if constexpr (!WIDENED<T>) {
+            if (bn * bm >= 128 && K >= 1280 && K % 16 == 0 && aligned16(x) && aligned16(w)) {
+                const unsigned blocks = (unsigned)((bn * bm + 7) / 8 * 8);
+                linear_big_kernel<T><<<dim3(blocks), 256, 0, s>>>(g, (int)bn, (int)bm);
+                return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
             }
         }
-        return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
+        return in_parts(TILE, [&](const LinearArgs& h, unsigned count) {
+            linear_tile_kernel<T><<<dim3((unsigned)tn, count), 256, 0, s>>>(h);
+        });
     });
 }

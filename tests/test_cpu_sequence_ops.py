@@ -102,6 +102,8 @@ def test_c_entry_points_refuse_before_launching():
     assert lib.kvae_linear_8bit(2, 8, 4, one, None, one, one, None, 0, one, None) == -1
     assert lib.kvae_linear_8bit(2, 8, 4, one, one, one, one, None, 1, one, None) == -2
     assert lib.kvae_linear_8bit(2, 1 << 31, 4, one, one, one, one, None, 0, one, None) == -5
+    assert lib.kvae_linear_8bit(2, 4, (1 << 22) + 1, one, one, one, one, None, 0, one, None) == -5
+    assert lib.kvae_linear_8bit((1 << 31) + 1, 4, 4, one, one, one, one, None, 0, one, None) == -5
 
 
 def test_segments_of_the_time_axis():

@@ -62,7 +62,7 @@ def test_sizes(M, N, K):
     check(kv.linear_8bit(x, sx, w, sw), x, sx, w, sw, None)
 
 
-@pytest.mark.parametrize("M,N,K", [(3, 40, 100), (40, 300, 520), (1000, 384, 256), (513, 1025, 777), (2000, 512, 1024),
+@pytest.mark.parametrize("M,N,K", [(3, 40, 100), (40, 300, 520), (1000, 384, 256), (513, 1025, 777), (2000, 512, 1024), (1100, 1030, 1),
                                    (700, 1300, 272)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_types(M, N, K, dtype):
@@ -86,8 +86,8 @@ def test_whole_numbers_are_exact():
         assert torch.equal(y.double(), a.double() @ b.double().t().contiguous())
 
 
-@pytest.mark.parametrize("M,N,K", [(2816, 2816, 16), (2817, 2900, 48), (4096, 2048, 64), (3000, 3000, 128), (2600, 3333, 176),
-                                   (5000, 1793, 208), (2304, 3328, 1040)])
+@pytest.mark.parametrize("M,N,K", [(2816, 2816, 1280), (2817, 2900, 1296), (4096, 2048, 1344), (3000, 3000, 1408), (2600, 3333, 1456),
+                                   (5000, 1793, 1312), (2304, 3328, 2000), (2900, 2900, 1295), (1300, 1300, 640)])
 def test_large_tiles(M, N, K):
     """Enough 256 x 256 tiles for the large form, ragged in rows, columns and k; NaN behind the rows."""
     import kalman_vae_amd as kv
