@@ -18,6 +18,8 @@
 // through LDS, the next k slice on its way while the present one is multiplied.
 #include "narrow_types.h"
 
+#include "device_info.h"
+
 namespace kvae {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
@@ -102,57 +104,79 @@ __device__ __forceinline__ void store4(const LinearArgs& g, long m, int n, const
     }
 }
 
-// Results of 32 rows by WN columns that a wavefront holds as WN / 32 sums of a 32 x 32 instruction:
-// a lane has row lane % 32, columns 32 i + 8 q + 4 (lane / 32) .. + 3.  Written from there, an
-// instruction would touch 32 rows with 16 bytes each; they go through LDS (`region`: the wavefront's own,
-// 32 rows) and out in runs of a whole row of WN.  value(i, e): element e of sum i.
-template <typename T, int WN, typename F>
-__device__ __forceinline__ void write_rows(const LinearArgs& g, char* region, long m0, int n0, int lane, F&& value) {
+// A tile's scales and biases in LDS, asked for at the start and there when the results go out.
+template <int ROWS>
+struct Factors {
+    float sx[ROWS], sw[ROWS], bias[ROWS];
+};
+template <int ROWS>
+__device__ __forceinline__ void load_factors(const LinearArgs& g, long m0, int n0, Factors<ROWS>& f) {
+    const int i = threadIdx.x;
+    if (i < ROWS) {
+        f.sx[i] = m0 + i < g.M ? g.sx[m0 + i] : 0.f;
+        f.sw[i] = n0 + i < g.N ? g.sw[n0 + i] : 0.f;
+        f.bias[i] = g.bias && n0 + i < g.N ? g.bias[n0 + i] : 0.f;
+    }
+}
+
+// Results of 32 JN rows by WN columns that a wavefront holds as JN x WN / 32 sums of a 32 x 32 instruction:
+// a lane has row 32 j + lane % 32, columns 32 i + 8 q + 4 (lane / 32) .. + 3.  Written from there, an
+// instruction would touch 32 rows with 16 bytes each; they go through LDS (`region`: the wavefront's own)
+// and out in runs of a whole row of WN.  rm, rn: first row and column inside the tile that starts at
+// (m0, n0); value(i, j, e): element e of sum (i, j).
+template <typename T, int WN, int JN, int ROWS, typename F>
+__device__ __forceinline__ void write_rows(const LinearArgs& g, const Factors<ROWS>& f, char* region, long m0, int n0,
+                                           int rm, int rn, int lane, F&& value) {
     constexpr int ROW = WN * (int)sizeof(T), CHUNKS = ROW / 16, PER = 16 / (int)sizeof(T);
-    const int row = lane & 31;
-    const long last = g.M - 1;
-    const float sx = g.sx[m0 + row < last ? m0 + row : last];
+    const int row = lane & 31, half = lane >> 5;
+    float sx[JN];
+#pragma unroll
+    for (int j = 0; j < JN; ++j) sx[j] = f.sx[rm + 32 * j + row];
 #pragma unroll
     for (int i = 0; i < WN / 32; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int in = 32 * i + 8 * q + 4 * (lane >> 5), n = n0 + in;
-            Pack<float, 4> sw{}, b{};
-            if (n + 4 <= g.N) {
-                sw = load_pack<float, 4>(g.sw + n);
-                if (g.bias) b = load_pack<float, 4>(g.bias + n);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < g.N) {
-                        sw.v[e] = g.sw[n + e];
-                        if (g.bias) b.v[e] = g.bias[n + e];
-                    }
-            }
-            Pack<T, 4> p;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p.v[e] = narrow<T>(value(i, 4 * q + e) * sx * sw.v[e] + b.v[e]);
+            const int in = 32 * i + 8 * q + 4 * half;
+            const v4f sw = *reinterpret_cast<const v4f*>(f.sw + rn + in);
+            const v4f b = *reinterpret_cast<const v4f*>(f.bias + rn + in);
             // (the exclusive-or spreads the rows over the banks)
             const int chunk = in / PER ^ (row & (CHUNKS - 1));
-            *reinterpret_cast<Pack<T, 4>*>(region + row * ROW + chunk * 16 + in % PER * (int)sizeof(T)) = p;
+            char* at = region + row * ROW + chunk * 16 + in % PER * (int)sizeof(T);
+#pragma unroll
+            for (int j = 0; j < JN; ++j) {
+                Pack<T, 4> p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p.v[e] = narrow<T>(value(i, j, 4 * q + e) * sx[j] * sw[e] + b[e]);
+                *reinterpret_cast<Pack<T, 4>*>(at + 32 * j * ROW) = p;
+            }
         }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    constexpr int ROWS = 64 / CHUNKS;                // rows of one instruction
-    T* y = static_cast<T*>(g.y);
+    constexpr int STEP = 64 / CHUNKS;                // rows of one instruction
+    const int r0 = lane / CHUNKS, c = lane % CHUNKS;
+    const long m = m0 + rm;
+    const int n = n0 + rn + c * PER;
+    T* out = static_cast<T*>(g.y) + (m + r0) * g.N + n;
+    const auto piece = [&](int k) {
+        const int r = k * STEP + r0;
+        return *reinterpret_cast<const Pack<T, PER>*>(region + r * ROW + (c ^ (r & (CHUNKS - 1))) * 16);
+    };
+    if (m + 32 * JN <= g.M && n0 + rn + WN <= g.N) {
 #pragma unroll
-    for (int k = 0; k < 32 / ROWS; ++k) {
-        const int r = k * ROWS + lane / CHUNKS, c = lane % CHUNKS, n = n0 + c * PER;
-        const Pack<T, PER> p = *reinterpret_cast<const Pack<T, PER>*>(region + r * ROW + (c ^ (r & (CHUNKS - 1))) * 16);
-        if (m0 + r < g.M) {
-            T* out = y + (m0 + r) * g.N + n;
+        for (int k = 0; k < 32 * JN / STEP; ++k) store_pack<T, PER>(out + (long)k * STEP * g.N, piece(k));
+    } else {
+#pragma unroll 1
+        for (int k = 0; k < 32 * JN / STEP; ++k) {
+            const Pack<T, PER> p = piece(k);
+            T* at = out + (long)k * STEP * g.N;
+            if (m + k * STEP + r0 >= g.M) continue;
             if (n + PER <= g.N) {
-                store_pack<T, PER>(out, p);
+                store_pack<T, PER>(at, p);
             } else {
 #pragma unroll
                 for (int e = 0; e < PER; ++e)
-                    if (n + e < g.N) out[e] = p.v[e];
+                    if (n + e < g.N) at[e] = p.v[e];
             }
         }
     }
@@ -226,6 +250,7 @@ __device__ __forceinline__ int piece_at(int r, int c) { return r * (SLICE / 16) 
 template <typename T>
 __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
     __shared__ v4i shared[2 * TILE * SLICE / 16];
+    __shared__ Factors<TILE> factors;
     v4i *xs = shared, *ws = shared + TILE * SLICE / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long m0 = (long)blockIdx.y * TILE;
@@ -300,6 +325,7 @@ __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
         }
     };
     fetch(0);
+    load_factors(g, m0, n0, factors);                // (read behind the loop's barriers)
     for (int s = 0; s < slices; ++s) {
         if ((s + 1) * SLICE > g.K) {
             const int behind = s * SLICE + col + 16 - g.K;
@@ -323,7 +349,8 @@ __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
     char* region = reinterpret_cast<char*>(shared) + wave * (32 * 64 * (int)sizeof(T));
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-        write_rows<T, 64>(g, region, m0 + wm + 32 * j, n0 + wn, lane, [&](int i, int e) { return acc[i][j][e]; });
+        write_rows<T, 64, 1>(g, factors, region, m0, n0, wm + 32 * j, wn, lane,
+                             [&](int i, int, int e) { return acc[i][j][e]; });
 }
 
 // Large products: 256 x 256 tiles, four wavefronts of 128 x 128 each (their sums fill the accumulation
@@ -331,21 +358,24 @@ __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
 // (1024 cycles) per wavefront on eight operands of 2 KB, so that the four wavefronts ask LDS for 64 bytes
 // a cycle, half of what 64 x 64 wavefront tiles would.
 //
-// Slices go from memory straight into LDS (no registers in between), into four buffers in turn: while
-// slice s is multiplied, the operands of s + 1 are read into registers of their own and s + 2 and s + 3 are
-// on their way.  One barrier per slice: a wavefront waits until its own pieces of s + 1 have arrived, and
-// behind the barrier everybody's have; the buffer that s + 3 goes to held s - 1, whose operands everybody
-// had read before.
+// Double slices (128 bytes of each row: whole cache lines) go from memory straight into LDS, no registers
+// in between, into two buffers in turn, and are multiplied half by half: while a half is multiplied, the
+// operands of the next half are read into registers of their own.  When the second half of one double
+// slice has been read by everybody, the double slice after next is asked for into its place: it has two
+// steps (2048 cycles) to arrive.  One barrier per double slice, before its first half is read: a wavefront
+// waits there until its own pieces have arrived, and behind the barrier everybody's have. 
 //
 // Rows that are not there repeat the last one (their results are not stored).  Where k ends inside the
 // last slice, pieces behind the end repeat the row's last piece and are replaced by zero on their way
 // from LDS to the registers, in both operands (a NaN in one of them must not meet the other's zero).
-constexpr int BIG = 256, BIG_SLICE = 64, BUFFERS = 4;
-constexpr int OPERAND = BIG * BIG_SLICE / 16;        // pieces of one operand's slice
+constexpr int BIG = 256, BIG_SLICE = 128;
+constexpr int OPERAND = BIG * BIG_SLICE / 16;        // pieces of one operand's double slice
 
 template <typename T>
 __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int tiles_n, int tiles_m) {
-    __shared__ v4i lds[BUFFERS * 2 * OPERAND];       // [buffer][x, w][row][4 pieces, see below]: 128 KB
+    static_assert(sizeof(T) == 2, "four wavefronts' results fill the LDS");
+    __shared__ v4i lds[2 * 2 * OPERAND];             // [buffer][x, w][row][8 pieces, see below]: 128 KB
+    __shared__ Factors<BIG> factors;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go round the eight dies (blockIdx % 8): each die gets a run of neighbouring tiles, in
     // groups of eight rows of tiles, so that its cache serves the tiles that run together.
@@ -358,25 +388,25 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
     const int n0 = rest / rows * BIG;
     const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
 
-    // Piece c of row r lies at place c ^ (r / 4 % 4) of the row, which spreads a column of pieces over
-    // the banks.  An instruction moves 16 rows: lane l fills place l % 4 of row l / 4.
-    const int piece = (lane & 3) ^ ((lane >> 4) & 3), last_piece = g.K / 16 - 1;
+    // Piece c of row r lies at place c ^ (r % 8) of the row, which spreads a column of pieces over the
+    // banks.  An instruction moves 8 rows: lane l fills place l % 8 of row l / 8.
+    const int piece = (lane & 7) ^ (lane >> 3), last_piece = g.K / 16 - 1;
     const uint8_t* xb = g.x + m0 * g.K;
     const uint8_t* wb = g.w + (long)n0 * g.K;
     const long rows_x = g.M - m0, rows_w = g.N - n0;
-    unsigned x_row[4], w_row[4];                     // byte offsets of the lane's rows
+    unsigned x_row[8], w_row[8];                     // byte offsets of the lane's rows
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long r = 16 * (wave + 4 * i) + (lane >> 2);
+    for (int i = 0; i < 8; ++i) {
+        const long r = 8 * (wave + 4 * i) + (lane >> 3);
         x_row[i] = (unsigned)(r < rows_x ? r : rows_x - 1) * (unsigned)g.K;
         w_row[i] = (unsigned)(r < rows_w ? r : rows_w - 1) * (unsigned)g.K;
     }
-    const auto fetch = [&](int s) {
-        const int p = 4 * s + piece;
+    const auto fetch = [&](int d) {                  // double slice d
+        const int p = 8 * d + piece;
         const unsigned k = 16u * (unsigned)(p < last_piece ? p : last_piece);
-        v4i* at = lds + (s % BUFFERS) * 2 * OPERAND + wave * 64;
+        v4i* at = lds + (d & 1) * 2 * OPERAND + wave * 64;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             __builtin_amdgcn_global_load_lds(
                 (const __attribute__((address_space(1))) void*)(xb + (x_row[i] + k)),
                 (__attribute__((address_space(3))) void*)(at + 256 * i), 16, 0, 0);
@@ -388,15 +418,16 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
     struct Operands {
         v8i a[4], b[4];
     };
-    const int turn = (lane >> 5) * 2 ^ ((lane >> 2) & 3), row4 = (lane & 31) * 4;
-    const auto read = [&](int s, Operands& h) {
-        const v4i* x = lds + (s % BUFFERS) * 2 * OPERAND + wm * 4 + row4;
-        const v4i* w = lds + (s % BUFFERS) * 2 * OPERAND + OPERAND + wn * 4 + row4;
+    const int row8 = (lane & 31) * 8;
+    const auto read = [&](int d, int half, Operands& h) {
+        const int turn = (half * 4 + (lane >> 5) * 2) ^ (lane & 7);
+        const v4i* x = lds + (d & 1) * 2 * OPERAND + wm * 8 + row8;
+        const v4i* w = lds + (d & 1) * 2 * OPERAND + OPERAND + wn * 8 + row8;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const v4i p = w[128 * t + turn], q = w[128 * t + (turn ^ 1)];
+            const v4i p = w[256 * t + turn], q = w[256 * t + (turn ^ 1)];
             h.a[t] = v8i{p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-            const v4i u = x[128 * t + turn], v = x[128 * t + (turn ^ 1)];
+            const v4i u = x[256 * t + turn], v = x[256 * t + (turn ^ 1)];
             h.b[t] = v8i{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
         }
     };
@@ -415,32 +446,32 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
                 acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(h.a[i], h.b[j], acc[i][j], 0, 0, 0,
                                                                             0, 0, 0);
     };
-    // Multiplies slice s from `now` and reads slice s + 1 into `next`.  The eight pieces that a wavefront
-    // asks for last (slice s + 2) may still be on their way, those of s + 1 may not, and its own reads of
-    // slice s are done (they were issued half a step ago or earlier).  The reads go between the first
-    // eight matrix instructions, the requests between the others.
-    const auto step = [&](int s, const Operands& now, Operands& next) {
-        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        read(s + 1, next);
-        fetch(s + 3);
-        multiply(now);
+    // Requests and reads go between the matrix instructions, requests first.
+    const auto interleave = [](bool requests) {
+        if (requests) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a matrix instruction
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // two reads
+            for (int i = 0; i < 8; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);   // two requests
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);   // a request
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);       // two reads
         }
+        if (!requests) __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    // zero where slice s is behind the end of k
-    const auto cut = [&](int s, Operands& h) {
-        const int there = g.K / 16 - 4 * s - (lane >> 5) * 2;
+    // everything asked for has arrived, for everybody, and everybody's reads are done
+    const auto arrive = [] {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // zero where half `half` of double slice d is behind the end of k
+    const auto cut = [&](int d, int half, Operands& h) {
+        const int there = g.K / 16 - 8 * d - 4 * half - (lane >> 5) * 2;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -449,35 +480,34 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
                 h.b[t][i] = there > i / 4 ? h.b[t][i] : 0;
             }
     };
-    // Slices are walked in pairs (one of zeros is added to an odd number), so that the loop is one
-    // straight run; what it fetches behind the end is not used.
-    const int pairs = (g.K + 2 * BIG_SLICE - 1) / (2 * BIG_SLICE);
+    // The last double slice is apart, as k may end in it; what the loop fetches behind the end is not used.
+    const int doubles = (g.K + BIG_SLICE - 1) / BIG_SLICE;
+    Operands first, second;
     fetch(0);
+    load_factors(g, m0, n0, factors);
+    arrive();
     fetch(1);
-    fetch(2);
-    Operands even, odd;
-    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    read(0, even);
-    for (int p = 0; p < pairs - 1; ++p) {
-        step(2 * p, even, odd);
-        step(2 * p + 1, odd, even);
+    read(0, 0, first);
+    for (int d = 0; d < doubles - 1; ++d) {
+        read(d, 1, second);
+        multiply(first);
+        interleave(false);
+        arrive();                                    // d + 1 is there, nobody reads d any more
+        fetch(d + 2);
+        read(d + 1, 0, first);
+        multiply(second);
+        interleave(true);
     }
-    const int s = 2 * (pairs - 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (nothing may still be written when others take over the LDS)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    read(s + 1, odd);
-    cut(s, even);
-    multiply(even);
-    cut(s + 1, odd);
-    multiply(odd);
+    arrive();                                        // (nothing may still be written when others take over the LDS)
+    read(doubles - 1, 1, second);
+    cut(doubles - 1, 0, first);
+    multiply(first);
+    cut(doubles - 1, 1, second);
+    multiply(second);
     __syncthreads();                                 // the operands' LDS is free
-    char* region = reinterpret_cast<char*>(lds) + wave * (32 * 128 * (int)sizeof(T));
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        write_rows<T, 128>(g, region, m0 + wm + 32 * j, n0 + wn, lane, [&](int i, int e) { return acc[i][j][e]; });
+    char* region = reinterpret_cast<char*>(lds) + wave * (128 * 128 * (int)sizeof(T));
+    write_rows<T, 128, 4>(g, factors, region, m0, n0, wm, wn, lane,
+                          [&](int i, int j, int e) { return acc[i][j][e]; });
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -504,9 +534,11 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
         // - up to 64 rows, k < 16, or fewer than 64 tiles of 128 x 128 (a quarter of the card's units): few rows.
         //   512^3 4.1 against 8.3 in tiles, 128 x 4096 x 4096 21 against 34; at 64 tiles (1024^3) 12 each,
         //   256 x 4096 x 4096 39 against 34.
-        // - half the card's units or more in tiles of 256 x 256, k long enough to hide that such a tile
-        //   neither starts nor ends under another one's work, and rows of whole 16-byte pieces: large tiles.
-        //   16384 x 4096 with k = 4096: 250 against 338 in tiles of 128; k = 1024: 107 against 97.
+        // - tiles of 256 x 256 that fill the card's units to seven eighths in every round, k long enough to
+        //   hide that such a tile neither starts nor ends under another one's work, and rows of whole
+        //   16-byte pieces: large tiles.  4096 x 4096 (256 of them) with k = 4096: 67 against 84 in tiles of
+        //   128; k = 1536, 16384 rows: 128 each; k = 1024: 100 against 92.  196 of them (3328 x 3328): 63
+        //   against 59.
         // (blockIdx.y is 16 bits: rows beyond go in further launches)
         const auto in_parts = [&](long rows_each, auto&& launch) {
             for (long first = 0; first < M; first += 65535 * rows_each) {
@@ -533,7 +565,8 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
             });
         }
         if constexpr (!WIDENED<T>) {
-            if (bn * bm >= 128 && K >= 1280 && K % 16 == 0 && aligned16(x) && aligned16(w)) {
+            const long units = device_compute_units(), rounds = (bn * bm + units - 1) / units;
+            if (bn * bm * 8 >= rounds * units * 7 && K >= 1536 && K % 16 == 0 && aligned16(x) && aligned16(w)) {
                 const unsigned blocks = (unsigned)((bn * bm + 7) / 8 * 8);
                 linear_big_kernel<T><<<dim3(blocks), 256, 0, s>>>(g, (int)bn, (int)bm);
                 return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
