@@ -238,8 +238,8 @@ KT_DEV bool chol(const Tile& S, Tile& LT, Tile& Li, float& diag) {
     static_assert(N % 8 == 0 && N <= 32, "tile shapes");
     typedef float f2 __attribute__((ext_vector_type(2)));
     const int i = lane_col(), h = lane_half();
-    // row i of S, then of L, as register pairs: the dot products below run on
-    // v_pk_fma_f32 with a pair of broadcast values as the scalar operand
+    // row i of S, then of L, as register pairs: the dot products below take a pair of
+    // broadcast values as scalar operands
     f2 row[N / 2];
     KT_UNROLL
     for (int r = 0; r < N / 2; ++r) {
