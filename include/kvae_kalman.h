@@ -698,7 +698,9 @@ int kvae_graph_count_kernel_nodes(void *hip_graph);
  * dtype: KVAE_F32, KVAE_BF16 or KVAE_F16 for u, y, dy, du; the state is float throughout.
  * u and dy have any strides over time and batch and stride 1 over the last axis; their address
  * needs the element's alignment only.  y (T,B,H), du (T,B,3H or 2H), h0, last, dlast, dh0 (B,H)
- * are contiguous and must not overlap the inputs.
+ * are contiguous and must not overlap the inputs.  KVAE_E_TOOLARGE where B H reaches 2^32, or where the
+ * sequences of one workgroup (B, or 512 / H + 2 if that is fewer) span 2^31 bytes in a tensor: batch
+ * strides of that size need a copy with smaller ones.
  * forward: writes y, last = c_{T-1} (or NULL) and, for a later backward call, states
  *   (ceil(T / L), B, H): c before every L-th step, L = KVAE_SCAN_CHUNK(dtype) (or NULL).
  * backward: reads u, mask, states, dy and dlast (or NULL); writes du and dh0 (or NULL).
@@ -776,7 +778,8 @@ int kvae_quantize_rows(int64_t rows, int64_t D, int dtype, const void *x, int64_
 /* Product of 8-bit rows, y (M,N) = (x w^T) * x_scale[m] * w_scale[n] + bias[n]: the projection that
  * reads kvae_rms_norm_quantized's output in the serving form of the "gated" network.  x (M,K) and
  * w (N,K) contiguous e4m3 bytes at any address, x_scale (M), w_scale (N) and bias (N, or NULL) float;
- * sums in float; y of out_dtype (KVAE_F32, KVAE_BF16 or KVAE_F16).  K up to 2^22.              */
+ * sums in float; y of out_dtype (KVAE_F32, KVAE_BF16 or KVAE_F16).  K up to 2^22, N up to 2^26,
+ * M up to 2^31, M N up to 2^40.                                                             */
 int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void *x, const void *x_scale,
                      const void *w, const void *w_scale, const void *bias, int out_dtype, void *y,
                      void *stream);

@@ -279,7 +279,7 @@ extern "C" int kvae_adamw_step(const kvae_adamw* d, void* stream) {
         g.first_block[i] = (unsigned)blocks;
         chunks += (t.numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
         blocks += (t.numel + QUANT_BLOCK - 1) / QUANT_BLOCK;
-        if (chunks > 0x7fffffffL) return KVAE_E_TOOLARGE;
+        if (chunks >= (1L << 32) / ADAM_THREADS) return KVAE_E_TOOLARGE;   // a launch has fewer than 2^32 threads
     }
     g.first_chunk[d->count] = (int)chunks;
     g.count = d->count;

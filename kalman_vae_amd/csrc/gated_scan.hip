@@ -618,12 +618,15 @@ static Plan scan_plan(long T, long B, long H, int dtype) {
     return p;
 }
 
+// a launch has fewer than 2^32 threads, and a channel has up to four (wavefronts that share the time axis
+// only do so where there are few channels)
+constexpr long MOST_CHANNELS = (1L << 32) - SCAN_BLOCK;
+
 static int check_scan(const kvae_gated_scan* d) {
     if (!d || d->T < 1 || d->B < 1 || d->H < 1 || !d->u) return KVAE_E_BADARG;
     if (d->dtype != KVAE_F32 && d->dtype != KVAE_BF16 && d->dtype != KVAE_F16)
         return KVAE_E_UNSUPPORTED;
-    // a workgroup holds at least 64 lanes and blockIdx.x is 31 bits
-    if (d->B > (1L << 36) / d->H) return KVAE_E_TOOLARGE;
+    if (d->B > MOST_CHANNELS / d->H) return KVAE_E_TOOLARGE;
     // lane offsets are 32 bits: the sequences of a workgroup (up to 256 lanes of one channel) must
     // lie within 2^31 bytes of each other
     if (d->u_stride_b < 0 || d->dy_stride_b < 0 || d->mask_stride_b < 0) return KVAE_E_BADARG;
@@ -676,7 +679,8 @@ static void with_bool(bool x, F&& f) {
 
 template <bool BACKWARD>
 static int run_scan(const kvae_gated_scan* d, void* workspace, size_t bytes, hipStream_t stream) {
-    if (bytes < kvae_gated_scan_workspace_bytes(d->T, d->B, d->H, d->dtype)) return KVAE_E_WORKSPACE;
+    const size_t need = kvae_gated_scan_workspace_bytes(d->T, d->B, d->H, d->dtype);
+    if (bytes < need || (need && !workspace)) return KVAE_E_WORKSPACE;
     const Plan plan = scan_plan(d->T, d->B, d->H, d->dtype);
     ScanArgs g = scan_args(d);
     g.seg = plan.seg, g.segs = plan.segs;
@@ -729,7 +733,7 @@ extern "C" int kvae_gated_scan_step(int64_t B, int64_t H, int dtype, int gated, 
                                     int64_t u_stride_b, const void* mask, int64_t mask_stride_b,
                                     void* state, void* y, void* stream) {
     if (B < 1 || H < 1 || !u || !state || !y) return KVAE_E_BADARG;
-    if (B > (1L << 38) / H) return KVAE_E_TOOLARGE;
+    if (B > MOST_CHANNELS / H) return KVAE_E_TOOLARGE;
     return for_element_type(dtype, [&](auto e) {
         using T = decltype(e);
         constexpr int V = 4;

@@ -520,8 +520,8 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
                                 const void* w, const void* w_scale, const void* bias, int out_dtype,
                                 void* y, void* stream) {
     if (M < 1 || N < 1 || K < 1 || !x || !x_scale || !w || !w_scale || !y) return KVAE_E_BADARG;
-    // 32-bit offsets inside a tile of 256 rows, 31-bit numbers of tiles
-    if (N > (1 << 30) || K > (1 << 22) || M > (1L << 31) || M > (1L << 44) / N) return KVAE_E_TOOLARGE;
+    // 32-bit offsets inside a tile of 256 rows, fewer than 2^32 threads in a launch (512 for 16 columns)
+    if (N > (1 << 26) || K > (1 << 22) || M > (1L << 31) || M > (1L << 40) / N) return KVAE_E_TOOLARGE;
     return for_element_type(out_dtype, [&](auto e) {
         using T = decltype(e);
         const LinearArgs g{(long)M, (int)N, (int)K, static_cast<const uint8_t*>(x),

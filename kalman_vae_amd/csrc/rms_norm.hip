@@ -381,14 +381,26 @@ static NormArgs norm_args(const kvae_rms_norm* d) {
 }
 
 template <bool QUANT, bool NORM>
-static int run_forward(int dtype, const NormArgs& g, hipStream_t stream) {
+static int run_forward(int dtype, const NormArgs& all, hipStream_t stream) {
     return for_element_type(dtype, [&](auto e) {
         using T = decltype(e);
-        return with_shape<T>(g.D, [&](auto lpr, auto n) {
+        return with_shape<T>(all.D, [&](auto lpr, auto n) {
             constexpr int LPR = decltype(lpr)::value, N = decltype(n)::value;
             constexpr int BLOCK = norm_block<LPR>(), RPB = BLOCK / LPR;
-            norm_forward_kernel<T, LPR, N, QUANT, NORM>
-                <<<dim3((unsigned)((g.rows + RPB - 1) / RPB)), BLOCK, 0, stream>>>(g);
+            // (a launch has fewer than 2^32 threads: rows beyond go in further launches)
+            constexpr long MOST = (1L << 31) / LPR;
+            for (long first = 0; first < all.rows; first += MOST) {
+                NormArgs g = all;
+                g.rows = all.rows - first < MOST ? all.rows - first : MOST;
+                g.x = static_cast<const T*>(all.x) + first * all.x_row;
+                if (all.residual) g.residual = static_cast<const T*>(all.residual) + first * all.residual_row;
+                g.y = static_cast<char*>(all.y) + first * all.D * (QUANT ? 1 : (long)sizeof(T));
+                if (all.scale) g.scale = all.scale + first;
+                if (all.sum) g.sum = static_cast<T*>(all.sum) + first * all.D;
+                if (all.rstd) g.rstd = all.rstd + first;
+                norm_forward_kernel<T, LPR, N, QUANT, NORM>
+                    <<<dim3((unsigned)((g.rows + RPB - 1) / RPB)), BLOCK, 0, stream>>>(g);
+            }
             return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
         });
     });

@@ -7,11 +7,12 @@
 #include <dlfcn.h>
 
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
-#include <unordered_set>
+#include <initializer_list>
 #include <vector>
 
 #include "../../include/kvae_kalman.h"
@@ -97,14 +98,23 @@ void changed(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// Gradients of a gradient are refused when they are asked for, not when the graph is built.
-variable_list once_differentiable(variable_list grads) {
+// Gradients of a gradient are refused when they are asked for, not when the graph is built: the first
+// ones lead to what they were made from (so that no request passes them by) through a node that raises.
+struct DifferentiableOnce : public torch::autograd::Node {
+    variable_list apply(variable_list&&) override {
+        TORCH_CHECK(false, "trying to differentiate twice a function that is differentiable once");
+    }
+};
+variable_list once_differentiable(variable_list grads, const variable_list& made_from) {
     if (!at::GradMode::is_enabled()) return grads;
-    auto node = std::make_shared<torch::autograd::DelayedError>(
-        "trying to differentiate twice a function that is differentiable once", (int64_t)grads.size());
-    for (auto& g : grads)
-        if (g.defined()) g = g.detach().requires_grad_(true);
-    return (*node)(std::move(grads));
+    const auto node = std::make_shared<DifferentiableOnce>();
+    node->set_next_edges(torch::autograd::collect_next_edges(made_from));
+    for (auto& g : grads) {
+        if (!g.defined()) continue;
+        g = g.detach();
+        torch::autograd::set_history(g, node);
+    }
+    return grads;
 }
 
 // -- gated recurrence -------------------------------------------------------------------------
@@ -118,6 +128,19 @@ kvae_gated_scan scan_struct(const Tensor& u, const OptTensor& mask, bool gated) 
         d.mask_stride_t = mask->stride(0), d.mask_stride_b = mask->stride(1);
     }
     return d;
+}
+
+// f() with the tensors as they are or, where their batch strides are too wide for the kernels, copied.
+template <typename F>
+void with_strides(kvae_gated_scan& d, const Tensor& u, const OptTensor& mask, const Tensor& dy, F&& f) {
+    int rc = f();
+    if (rc != KVAE_E_TOOLARGE) return check(rc);
+    const Tensor u2 = u.contiguous(), m2 = mask && mask->defined() ? mask->contiguous() : Tensor(),
+                 dy2 = dy.defined() ? dy.contiguous() : Tensor();
+    d.u = u2.data_ptr(), d.u_stride_t = u2.stride(0), d.u_stride_b = u2.stride(1);
+    if (m2.defined()) d.mask = m2.data_ptr(), d.mask_stride_t = m2.stride(0), d.mask_stride_b = m2.stride(1);
+    if (dy2.defined()) d.dy = dy2.data_ptr(), d.dy_stride_t = dy2.stride(0), d.dy_stride_b = dy2.stride(1);
+    check(f());
 }
 
 Tensor scan_workspace(const kvae_gated_scan& d, const Tensor& like) {
@@ -134,7 +157,8 @@ std::array<Tensor, 3> scan_forward(const Tensor& u, const OptTensor& h0, const O
     d.h0 = address(h0), d.y = out[0].data_ptr(), d.last = out[1].data_ptr();
     d.states = keep ? out[2].data_ptr() : nullptr;
     const Tensor ws = scan_workspace(d, u);
-    check(lib.scan_forward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream));
+    with_strides(d, u, mask, Tensor(),
+                 [&] { return lib.scan_forward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream); });
     return out;
 }
 
@@ -164,9 +188,10 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
             d.dy = dy.data_ptr(), d.dy_stride_t = dy.stride(0), d.dy_stride_b = dy.stride(1);
             d.dlast = address(dlast), d.du = out[0].data_ptr(), d.dh0 = address(out[1]);
             const Tensor ws = scan_workspace(d, u);
-            check(lib.scan_backward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream));
+            with_strides(d, u, mask, dy,
+                         [&] { return lib.scan_backward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream); });
         }
-        return once_differentiable(std::move(out));
+        return once_differentiable(std::move(out), {u, grads[0], grads[1]});
     }
 };
 
@@ -251,7 +276,8 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
             check(lib.norm_backward(&d, on.stream));
             if (ctx->saved_data["residual"].toBool()) out[2] = out[0];
         }
-        return once_differentiable(std::move(out));
+        grads.insert(grads.end(), {x, residual, weight});
+        return once_differentiable(std::move(out), grads);
     }
 };
 
@@ -338,6 +364,28 @@ void check_list(const char* name, const std::vector<const Tensor*>& list, const 
     }
 }
 
+// Tensors that are written may not share memory: not the same one twice, not two views that overlap.
+void check_apart(std::initializer_list<const std::vector<const Tensor*>*> lists) {
+    struct Range {
+        const char *begin, *end;
+        bool operator<(const Range& o) const { return begin < o.begin; }
+    };
+    std::vector<Range> ranges;
+    for (const auto* list : lists) {
+        ranges.reserve(ranges.size() + list->size());
+        for (const Tensor* t : *list)
+            if (t->numel()) {
+                const char* at = static_cast<const char*>(t->data_ptr());
+                ranges.push_back({at, at + t->nbytes()});
+            }
+    }
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i)
+        TORCH_CHECK_VALUE(ranges[i].begin >= ranges[i - 1].end,
+                          "parameters, states and masters may not share memory: one of them appears twice in the "
+                          "lists, or two are views that overlap");
+}
+
 void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::object v_in, py::object step,
                 py::object lr, double beta1, double beta2, double eps, double weight_decay, py::object masters_in,
                 int64_t seed) {
@@ -347,9 +395,6 @@ void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::
     kvae_adamw d{};
     d.dtype = dtype_code(type);
     check_list("parameters", params, params, type);
-    std::unordered_set<const void*> seen;
-    for (const Tensor* p : params)
-        TORCH_CHECK_VALUE(p->numel() == 0 || seen.insert(p->data_ptr()).second, "a parameter appears twice in the list");
     const auto grads = list_of(grads_in, "gradients");
     check_list("gradients", grads, params, type);
     bool pairs = false, plain = false;
@@ -403,6 +448,7 @@ void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::
     } else {
         d.lr = lr.cast<double>();
     }
+    check_apart({&params, &m, &v, &ms, &vs, &masters});
     TORCH_CHECK(first.is_cuda(), "kalman_vae_amd runs on MI355X only: got a tensor on ", first.device(),
                 "; there is no CPU fallback");
     const On on(first);

@@ -24,11 +24,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
         p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
 
     ``params`` and ``grads``: contiguous GPU tensors of one type (float32, bfloat16 or float16) on one
-    device.  ``exp_avgs`` and ``exp_avg_sqs``: float32 tensors holding m and v, or pairs
+    device; none of the tensors that are written may share memory.  ``exp_avgs`` and ``exp_avg_sqs``: float32 tensors holding m and v, or pairs
     ``(codes, scales)`` holding m and sqrt(v) in 8 bits: codes of torch.float8_e4m3fn with the
     parameter's number of elements and one float32 scale per 256 of them (``state_blocks``).  8-bit
     states are rounded stochastically by a hash of ``seed``, ``step`` and the element's place in the
-    list: the same call gives the same bits.  ``masters``: float32 copies of 16-bit parameters that take the update, of which the
+    list: the same call gives the same bits.  A gradient that is not finite spoils the states of its
+    element (32 bits) or of its 256 (8 bits), so such an update has to be left out.  ``masters``: float32 copies of 16-bit parameters that take the update, of which the
     parameter is the rounded value; without them the update is rounded to the parameter's type.
 
     ``step``: the number of this update, from 1; or an int64 tensor of one element on the device that

@@ -66,7 +66,8 @@ def gated_scan(u, h0=None, mask=None, output_gate=True):
     step is skipped (the state passes through, y is 0, no gradient, whatever u holds there), so a
     padded batch ends in each sequence's own last state, and a sequence without any step in ``h0``.
     ``u`` may have any strides over time and batch (a batch-first tensor transposed, a slice of a
-    wider one) without a copy.  T = 0 returns ``h0`` as the last state.
+    wider one) without a copy, unless sequences that a workgroup takes together (up to 512 / H + 2)
+    lie 2^31 bytes apart.  T = 0 returns ``h0`` as the last state.
 
     Differentiable (once) with respect to ``u`` and ``h0``.  The backward pass reads u and the
     gradients and a float32 state per 16 steps that the forward pass keeps; the state and every sum

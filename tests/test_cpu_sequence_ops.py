@@ -187,3 +187,37 @@ def test_adamw_c_entry_point_refuses_before_launching():
     assert call([row()], state_bits=4) == -2 and call([row()], dtype=capi.KVAE_F64) == -2
     assert lib.kvae_adamw_step(None, None) == -1
     assert call([row(1 << 45)]) == -5
+
+
+def test_limits_of_a_launch_are_refused():
+    """A launch has fewer than 2^32 threads and its lanes 32-bit offsets: what does not fit is refused
+    before anything is launched, whatever the addresses (never followed here)."""
+    lib, one = capi.load(), 4096
+    d = capi.GatedScan(T=1, B=1 << 31, H=2, dtype=capi.KVAE_F32, gated=1, u=one, y=one, u_stride_b=6, u_stride_t=6)
+    assert lib.kvae_gated_scan_forward(C.byref(d), None, 0, None) == -5
+    assert lib.kvae_gated_scan_step(1 << 31, 2, 0, 1, one, 6, None, 0, one, one, None) == -5
+    for code, size in ((capi.KVAE_F32, 4), (capi.KVAE_BF16, 2)):
+        for name, width in (("u", size), ("mask", 1)):
+            d = capi.GatedScan(T=1, B=2, H=2, dtype=code, gated=1, u=one, y=one, mask=one, u_stride_b=6, u_stride_t=6)
+            setattr(d, name + "_stride_b", (1 << 31) // width + 1)
+            assert lib.kvae_gated_scan_forward(C.byref(d), None, 0, None) == -5, name
+    d = capi.GatedScan(T=1 << 20, B=2, H=8, dtype=capi.KVAE_F32, gated=1, u=one, y=one, u_stride_b=24, u_stride_t=48)
+    need = lib.kvae_gated_scan_workspace_bytes(d.T, d.B, d.H, d.dtype)
+    assert lib.kvae_gated_scan_forward(C.byref(d), None, need, None) == -3
+    assert lib.kvae_linear_8bit(2, (1 << 26) + 1, 4, one, one, one, one, None, 0, one, None) == -5
+    assert lib.kvae_linear_8bit(1 << 20, 1 << 21, 4, one, one, one, one, None, 0, one, None) == -5
+    assert lib.kvae_quantize_rows(1 << 31, 8, 0, one, 8, one, one, None) == -5
+
+
+def test_adamw_refuses_memory_that_is_written_twice():
+    from kalman_vae_amd import adamw_step
+    z = lambda n=4: torch.zeros(n)  # noqa: E731
+    flat, state = z(10), z()
+    for args in (([flat[:4], flat[3:7]], [z(), z()], [z(), z()], [z(), z()], 1),       # views that overlap
+                 ([z(), z()], [z(), z()], [state, state], [z(), z()], 1),              # one state for two
+                 ([z()], [z()], [state], [state], 1),                                  # m and v the same
+                 ([state], [z()], [state], [z()], 1)):                                 # m is the parameter
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step(*args)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):                         # neighbours are fine
+        adamw_step([flat[:4], flat[4:8]], [z(), z()], [z(), z()], [z(), z()], 1)
