@@ -76,11 +76,24 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 struct Place {
     long b0;
     unsigned b, h;
+    unsigned seg;                // segment of the time axis
 };
+// Workgroups go round the eight dies (id % 8).  With segments each die gets a run of neighbouring channel
+// groups: a group of 64 lanes begins anywhere in a 128-byte line, and the line that two of them share is
+// then fetched into one cache (32768 steps of 520 half channels: 19 -> 17 us to compose, 28 -> 26 to run).
+// Without, a whole sequence passes before its neighbour is far behind or ahead, and there is nothing to gain.
 template <int V, int W>
 __device__ __forceinline__ Place scan_place(const ScanArgs& g) {
-    const long first = (long)blockIdx.x * (W == 1 ? SCAN_BLOCK : 64);
     Place p;
+    p.seg = 0;
+    long first = (long)blockIdx.x * (W == 1 ? SCAN_BLOCK : 64);
+    if (W > 1 && g.segs > 1) {
+        const unsigned id = blockIdx.y * gridDim.x + blockIdx.x, total = gridDim.x * gridDim.y;
+        const unsigned die = id & 7, each = total >> 3, longer = total & 7;
+        const unsigned mine = die * each + (die < longer ? die : longer) + (id >> 3);
+        p.seg = mine / gridDim.x;
+        first = (long)(mine - p.seg * gridDim.x) * 64;
+    }
     p.b0 = first / g.groups;
     const long left = g.B * g.groups - first;        // lanes from here to the last one
     unsigned lane = W == 1 ? threadIdx.x : threadIdx.x & 63;
@@ -126,17 +139,17 @@ struct Exchange {
     Map<V> m[W][64];
 };
 
-// State (or, REVERSE, gradient) that segment blockIdx.y starts from: `init`, then the maps of the
+// State (or, REVERSE, gradient) that a segment starts from: `init`, then the maps of the
 // segments that come before it in walking order.  With several wavefronts each takes every W-th of
 // them in one stretch and the stretches meet in LDS.
 template <int V, int W, bool REVERSE>
-__device__ __forceinline__ void segment_start(const ScanArgs& g, int wave, long at, const float* init, Exchange<V, W>* ex,
+__device__ __forceinline__ void segment_start(const ScanArgs& g, int seg, int wave, long at, const float* init, Exchange<V, W>* ex,
                                               float (&c)[V]) {
 #pragma unroll
     for (int v = 0; v < V; ++v) c[v] = init ? init[at + v] : 0.f;
     if (g.segs == 1) return;
     const long plane = g.B * g.H;
-    const int before = REVERSE ? g.segs - 1 - (int)blockIdx.y : (int)blockIdx.y;
+    const int before = REVERSE ? g.segs - 1 - seg : seg;
     const int each = (before + W - 1) / W;
     const int begin = wave * each < before ? wave * each : before;
     const int end = begin + each < before ? begin + each : before;
@@ -230,13 +243,13 @@ __global__ void __launch_bounds__(W == 1 ? SCAN_BLOCK : 64 * W, 4) scan_forward_
     const Place place = scan_place<V, W>(g);
     const int lane = threadIdx.x & 63;
     const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long t_begin = (long)blockIdx.y * g.seg;
+    const long t_begin = (long)place.seg * g.seg;
     const long t_end = t_begin + g.seg < g.T ? t_begin + g.seg : g.T;
     const long at = (place.b0 + place.b) * g.H + place.h, plane = g.B * g.H;
     const long at0 = place.b0 * g.H;                 // at = at0 + place.b H + place.h
     const unsigned inside = place.b * (unsigned)g.H + place.h;
     float c[V];
-    segment_start<V, W, false>(g, wave, at, g.h0, &ex[0], c);
+    segment_start<V, W, false>(g, (int)place.seg, wave, at, g.h0, &ex[0], c);
     int turn = 1;                                    // (segment_start has used ex[0])
     const auto chunk = [&](auto full, long t0, int n) {
         constexpr bool FULL = decltype(full)::value, SELECT = MASKED || !FULL;
@@ -342,7 +355,7 @@ __global__ void __launch_bounds__(64 * W) scan_compose_kernel(ScanArgs g) {
     __shared__ Exchange<V, W> ex;
     const Place place = scan_place<V, W>(g);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long t_first = (long)blockIdx.y * g.seg;
+    const long t_first = (long)place.seg * g.seg;
     const long t_last = t_first + g.seg < g.T ? t_first + g.seg : g.T;
     const long stretch = g.seg / W;                  // (a multiple of L)
     const long t_begin = t_first + wave * stretch < t_last ? t_first + wave * stretch : t_last;
@@ -394,7 +407,7 @@ __global__ void __launch_bounds__(64 * W) scan_compose_kernel(ScanArgs g) {
     for (int w = 1; w < W; ++w) all = then<V>(all, ex.m[BACKWARD ? W - 1 - w : w][lane]);
     const long at = (place.b0 + place.b) * g.H + place.h, plane = g.B * g.H;
 #pragma unroll
-    for (int v = 0; v < V; ++v) g.compose[blockIdx.y * plane + at + v] = make_float2(all.P[v], all.S[v]);
+    for (int v = 0; v < V; ++v) g.compose[place.seg * plane + at + v] = make_float2(all.P[v], all.S[v]);
 }
 
 // Adjoint.  carry = f_{t+1} G_{t+1}, the gradient that reaches c_t from later steps:
@@ -407,7 +420,7 @@ __global__ void __launch_bounds__(W == 1 ? SCAN_BLOCK : 64 * W, 4) scan_backward
     const Place place = scan_place<V, W>(g);
     const int lane = threadIdx.x & 63;
     const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long t_begin = (long)blockIdx.y * g.seg;
+    const long t_begin = (long)place.seg * g.seg;
     const long t_end = t_begin + g.seg < g.T ? t_begin + g.seg : g.T;
     const long at = (place.b0 + place.b) * g.H + place.h, plane = g.B * g.H;
     const long at0 = place.b0 * g.H;
@@ -415,7 +428,7 @@ __global__ void __launch_bounds__(W == 1 ? SCAN_BLOCK : 64 * W, 4) scan_backward
     const long row = (GATED ? 3 : 2) * g.H;
     const unsigned du_inside = (place.b * (unsigned)row + place.h) * (unsigned)sizeof(T);
     float carry[V];
-    segment_start<V, W, true>(g, wave, at, g.dlast, &ex[0], carry);
+    segment_start<V, W, true>(g, (int)place.seg, wave, at, g.dlast, &ex[0], carry);
     int turn = 1;
     const auto chunk = [&](auto full, long t0, int n) {
         constexpr bool FULL = decltype(full)::value, SELECT = MASKED || !FULL;
@@ -591,9 +604,10 @@ scan_step_kernel(long B, long H, const T* __restrict__ u, long u_b, const uint8_
 //   wavefronts and T = 1000: 57/90 against 135/210 alone; T = 20, 64 wavefronts: 4.4/6.8 against
 //   8.2/7.4.  (Eight: 5.1/8.7 there, and no faster on long sequences.)
 // - Fewer than 2048 with that: the sequence is cut into segments as well, up to 128, of at least two
-//   rounds of a workgroup each: 32768 steps of 520 half channels take 19 us to compose and 29 to
+//   rounds of a workgroup each: 32768 steps of 520 half channels take 17 us to compose and 26 to
 //   run (one wavefront per segment and a launch for the start states: 47 + 10 + 54).  u is read
-//   twice then.
+//   twice then.  (Asking for the next round's steps before a round is worked on: 21 + 30, and 1000
+//   masked steps 128 -> 235, as the barrier waits for what has been asked for.)
 struct Plan {
     int V, L, W, segs;
     long seg;                                        // steps per segment
