@@ -244,8 +244,12 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) linear_few_rows_kernel(LinearA
 }
 
 constexpr int TILE = 128, SLICE = 128;
-// LDS place of 16-byte piece c of row r: the exclusive-or spreads a column of pieces over the banks
-__device__ __forceinline__ int piece_at(int r, int c) { return r * (SLICE / 16) + (c ^ (r & 7)); }
+// LDS place of 16-byte piece c of row r.  A wavefront reads piece c of 32 rows with its lower lanes and
+// piece c + 1 with its upper lanes (which pieces a lane holds is free, as both operands share it); with
+// this exclusive-or such a read meets no bank twice.  (With r % 8, and pieces c and c + 2, a read took
+// 12 cycles of the LDS for 8: 16384 x 4096 x 1024 91 us against 82.)
+__device__ __forceinline__ int row_key(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int piece_at(int r, int c) { return r * (SLICE / 16) + (c ^ row_key(r)); }
 
 template <typename T>
 __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
@@ -279,13 +283,13 @@ __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
 #pragma unroll
         for (int s = 0; s < SLICE / 64; ++s) {
             v8i a[2], b[2];
-            const int c = s * 4 + (lane >> 5) * 2;
+            const int c = s * 4 + (lane >> 5);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int ra = wn + 32 * t + (lane & 31), rb = wm + 32 * t + (lane & 31);
-                const v4i p = ws[piece_at(ra, c)], q = ws[piece_at(ra, c + 1)];
+                const v4i p = ws[piece_at(ra, c)], q = ws[piece_at(ra, c + 2)];
                 a[t] = v8i{p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-                const v4i u = xs[piece_at(rb, c)], v = xs[piece_at(rb, c + 1)];
+                const v4i u = xs[piece_at(rb, c)], v = xs[piece_at(rb, c + 2)];
                 b[t] = v8i{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
             }
             if constexpr (WIDENED<T>) {
@@ -374,7 +378,11 @@ constexpr int OPERAND = BIG * BIG_SLICE / 16;        // pieces of one operand's 
 template <typename T>
 __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int tiles_n, int tiles_m) {
     static_assert(sizeof(T) == 2, "four wavefronts' results fill the LDS");
-    __shared__ v4i lds[2 * 2 * OPERAND];             // [buffer][x, w][row][8 pieces, see below]: 128 KB
+    // Two buffers of [x, w][row][8 pieces], 64 KB each.  They are two variables, and which one is meant is
+    // known where the code is compiled: the compiler lets a read of LDS wait for every request into the same
+    // variable that is under way (with one variable for both each half step waited for what it had just
+    // asked for: 16384 x 4096 x 4096 264 us).
+    __shared__ v4i buffer0[2 * OPERAND], buffer1[2 * OPERAND];
     __shared__ Factors<BIG> factors;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go round the eight dies (blockIdx % 8): each die gets a run of neighbouring tiles, in
@@ -388,9 +396,8 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
     const int n0 = rest / rows * BIG;
     const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
 
-    // Piece c of row r lies at place c ^ (r % 8) of the row, which spreads a column of pieces over the
-    // banks.  An instruction moves 8 rows: lane l fills place l % 8 of row l / 8.
-    const int piece = (lane & 7) ^ (lane >> 3), last_piece = g.K / 16 - 1;
+    // Pieces lie as in the small tiles.  An instruction moves 8 rows: lane l fills place l % 8 of row l / 8.
+    const int piece = (lane & 7) ^ row_key(8 * wave + (lane >> 3)), last_piece = g.K / 16 - 1;
     const uint8_t* xb = g.x + m0 * g.K;
     const uint8_t* wb = g.w + (long)n0 * g.K;
     const long rows_x = g.M - m0, rows_w = g.N - n0;
@@ -401,10 +408,11 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
         x_row[i] = (unsigned)(r < rows_x ? r : rows_x - 1) * (unsigned)g.K;
         w_row[i] = (unsigned)(r < rows_w ? r : rows_w - 1) * (unsigned)g.K;
     }
-    const auto fetch = [&](int d) {                  // double slice d
+    // `b`: std::integral_constant of the buffer
+    const auto fetch = [&](auto b, int d) {          // double slice d
         const int p = 8 * d + piece;
         const unsigned k = 16u * (unsigned)(p < last_piece ? p : last_piece);
-        v4i* at = lds + (d & 1) * 2 * OPERAND + wave * 64;
+        v4i* at = (decltype(b)::value ? buffer1 : buffer0) + wave * 64;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             __builtin_amdgcn_global_load_lds(
@@ -419,15 +427,15 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
         v8i a[4], b[4];
     };
     const int row8 = (lane & 31) * 8;
-    const auto read = [&](int d, int half, Operands& h) {
-        const int turn = (half * 4 + (lane >> 5) * 2) ^ (lane & 7);
-        const v4i* x = lds + (d & 1) * 2 * OPERAND + wm * 8 + row8;
-        const v4i* w = lds + (d & 1) * 2 * OPERAND + OPERAND + wn * 8 + row8;
+    const auto read = [&](auto b, int half, Operands& h) {
+        const int turn = (half * 4 + (lane >> 5)) ^ row_key(lane & 31);
+        const v4i* x = (decltype(b)::value ? buffer1 : buffer0) + wm * 8 + row8;
+        const v4i* w = (decltype(b)::value ? buffer1 : buffer0) + OPERAND + wn * 8 + row8;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const v4i p = w[256 * t + turn], q = w[256 * t + (turn ^ 1)];
+            const v4i p = w[256 * t + turn], q = w[256 * t + (turn ^ 2)];
             h.a[t] = v8i{p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-            const v4i u = x[256 * t + turn], v = x[256 * t + (turn ^ 1)];
+            const v4i u = x[256 * t + turn], v = x[256 * t + (turn ^ 2)];
             h.b[t] = v8i{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
         }
     };
@@ -465,47 +473,49 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
     };
     // everything asked for has arrived, for everybody, and everybody's reads are done
     const auto arrive = [] {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);          // vmcnt(0) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
     // zero where half `half` of double slice d is behind the end of k
     const auto cut = [&](int d, int half, Operands& h) {
-        const int there = g.K / 16 - 8 * d - 4 * half - (lane >> 5) * 2;
+        const int there = g.K / 16 - 8 * d - 4 * half - (lane >> 5);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                h.a[t][i] = there > i / 4 ? h.a[t][i] : 0;
-                h.b[t][i] = there > i / 4 ? h.b[t][i] : 0;
+                h.a[t][i] = there > i / 4 * 2 ? h.a[t][i] : 0;
+                h.b[t][i] = there > i / 4 * 2 ? h.b[t][i] : 0;
             }
     };
-    // The last double slice is apart, as k may end in it; what the loop fetches behind the end is not used.
     const int doubles = (g.K + BIG_SLICE - 1) / BIG_SLICE;
     Operands first, second;
-    fetch(0);
-    load_factors(g, m0, n0, factors);
-    arrive();
-    fetch(1);
-    read(0, 0, first);
-    for (int d = 0; d < doubles - 1; ++d) {
-        read(d, 1, second);
+    const auto step = [&](auto b, int d) {
+        constexpr std::integral_constant<int, 1 - decltype(b)::value> other{};
+        const bool ends = (d + 1) * BIG_SLICE > g.K;
+        if (ends) cut(d, 0, first);
+        read(b, 1, second);
         multiply(first);
         interleave(false);
+        if (ends) cut(d, 1, second);
         arrive();                                    // d + 1 is there, nobody reads d any more
-        fetch(d + 2);
-        read(d + 1, 0, first);
+        fetch(b, d + 2);                             // (behind the end of k: not used)
+        read(other, 0, first);
         multiply(second);
         interleave(true);
-    }
-    arrive();                                        // (nothing may still be written when others take over the LDS)
-    read(doubles - 1, 1, second);
-    cut(doubles - 1, 0, first);
-    multiply(first);
-    cut(doubles - 1, 1, second);
-    multiply(second);
-    __syncthreads();                                 // the operands' LDS is free
-    char* region = reinterpret_cast<char*>(lds) + wave * (128 * 128 * (int)sizeof(T));
+    };
+    constexpr std::integral_constant<int, 0> b0{};
+    constexpr std::integral_constant<int, 1> b1{};
+    fetch(b0, 0);
+    load_factors(g, m0, n0, factors);
+    arrive();
+    fetch(b1, 1);
+    read(b0, 0, first);
+    for (int d = 0; d < doubles; d += 2) step(b0, d), step(b1, d + 1);
+    arrive();                                        // nothing is under way, the operands' LDS is free
+    // (a wavefront's 32 KB lie in one of the buffers)
+    char* region = reinterpret_cast<char*>(wave < 2 ? buffer0 : buffer1) + (wave & 1) * (128 * 128 * (int)sizeof(T));
     write_rows<T, 128, 4>(g, factors, region, m0, n0, wm, wn, lane,
                           [&](int i, int j, int e) { return acc[i][j][e]; });
 }
