@@ -13,9 +13,18 @@
 // first operand's place: then a lane's results are four neighbouring n of one row m, which go out
 // as one wide store, and the matrix instruction's k order does not matter as both sides share it.
 //
-// Two forms.  Few rows: reading w once is the work, so a workgroup takes 16 rows of w straight into
-// registers, its wavefronts share out k and add up through LDS.  Many rows: 128 x 128 tiles staged
-// through LDS, the next k slice on its way while the present one is multiplied.
+// Three forms.  Few rows: reading w once is the work; a workgroup takes 16 rows of w and up to 64 of x, its
+// wavefronts share out k and add up through LDS.  Tiles of 128 x 128 staged through registers and LDS, the
+// next slice of k on its way while the present one is multiplied, three workgroups to a unit.  Large tiles of
+// 256 x 256, fed from memory straight into LDS, for large products.
+//
+// Measured (bfloat16 results): 1 x 6144 x 2048 4.3 us (2.9 TB/s), 64 x 4096 x 4096 6.8 us, 262144 x 384 x 128
+// 51 us (4.6 TB/s, memory's rate), 4096^3 58 us, 16384 x 4096 x 4096 220 us = 2.5 PFLOP/s, where the library's
+// product of 8-bit operands takes 224 us, and 8192^3 430 us = 2.6.  A loop of nothing but these instructions
+// reaches 3.4 to 4 on random bytes (the clock comes down).  Each round of large tiles spends some 12 us
+// outside its loop (first requests, results); workgroups that stay and ask for the next tile's start before
+// they write the last one's results were no faster (227 to 248 us), nor was a step that warms the second
+// cache two slices ahead (224 us).
 #include "narrow_types.h"
 
 #include "device_info.h"
@@ -61,10 +70,6 @@ __device__ __forceinline__ v4i load_piece(const uint8_t* row, int k, int K) {
 #pragma unroll 1
     for (int i = 0; k + i < K; ++i) (i < 8 ? lo : hi) |= (unsigned long)row[k + i] << (8 * (i & 7));
     return v4i{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
-}
-// the same, or zero where there is no such row
-__device__ __forceinline__ v4i load_chunk(const uint8_t* row, bool there, int k, int K) {
-    return load_piece(row, there ? k : K, K);
 }
 
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -185,64 +190,6 @@ __device__ __forceinline__ void write_rows(const LinearArgs& g, const Factors<RO
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-constexpr int FEW_WAVES = 8;
-// Rows of x: blockIdx.y * 16 MT ..., rows of w: blockIdx.x * 16 ...
-template <typename T, int MT>
-__global__ void __launch_bounds__(64 * FEW_WAVES) linear_few_rows_kernel(LinearArgs g) {
-    __shared__ float sums[FEW_WAVES][MT][64][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = lane & 15, part = (lane >> 4) * 32;
-    const long m0 = (long)blockIdx.y * 16 * MT;
-    const int n = blockIdx.x * 16 + row;
-    const bool has_n = n < g.N;
-    const uint8_t* w = g.w + (has_n ? (long)n * g.K : 0);
-    const uint8_t* x[MT];
-    bool has_m[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        has_m[t] = m0 + 16 * t + row < g.M;
-        x[t] = g.x + (has_m[t] ? (m0 + 16 * t + row) * (long)g.K : 0);
-    }
-    v4f acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = wave * 128; k0 < g.K; k0 += FEW_WAVES * 128) {
-        const int k = k0 + part;
-        const v4i a0 = load_chunk(w, has_n, k, g.K), a1 = load_chunk(w, has_n, k + 16, g.K);
-        const v8i a = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-        v8h ah[4];
-        if constexpr (WIDENED<T>) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ah[i] = widen8(a, i);
-        }
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const v4i b0 = load_chunk(x[t], has_m[t], k, g.K), b1 = load_chunk(x[t], has_m[t], k + 16, g.K);
-            const v8i b = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
-            if constexpr (WIDENED<T>) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[i], widen8(b, i), acc[t], 0, 0, 0);
-            } else {
-                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], 0, 0, 0, 0, 0, 0);
-            }
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sums[wave][t][lane][i] = acc[t][i];
-    __syncthreads();
-    for (int t = wave; t < MT; t += FEW_WAVES) {
-        float total[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int v = 0; v < FEW_WAVES; ++v)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) total[i] += sums[v][t][lane][i];
-        store4<T>(g, m0 + 16 * t + (lane & 15), blockIdx.x * 16 + 4 * (lane >> 4), total);
-    }
-}
-
 constexpr int TILE = 128, SLICE = 128;
 // LDS place of 16-byte piece c of row r.  A wavefront reads piece c of 32 rows with its lower lanes and
 // piece c + 1 with its upper lanes (which pieces a lane holds is free, as both operands share it); with
@@ -250,6 +197,101 @@ constexpr int TILE = 128, SLICE = 128;
 // 12 cycles of the LDS for 8: 16384 x 4096 x 1024 91 us against 82.)
 __device__ __forceinline__ int row_key(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int piece_at(int r, int c) { return r * (SLICE / 16) + (c ^ row_key(r)); }
+
+constexpr int FEW_WAVES = 8;
+// Rows of x: blockIdx.y * 16 MT ..., rows of w: blockIdx.x * 16 ...  The wavefronts share out k in slices of
+// 128 bytes.  The matrix instruction wants 16 rows side by side in 16 neighbouring lanes; loaded like that,
+// every lane would be in another cache line (57 cycles of the address unit for an instruction of 1 KB).
+// So eight lanes load a line, and the rows change lanes in LDS of the wavefront's own.
+template <typename T, int MT>
+__global__ void __launch_bounds__(64 * FEW_WAVES) linear_few_rows_kernel(LinearArgs g) {
+    constexpr int ROWS16 = 16 * SLICE / 16;          // pieces of 16 rows
+    __shared__ v4i lds[FEW_WAVES][(MT + 1) * ROWS16];
+    static_assert(sizeof(lds) >= FEW_WAVES * MT * 64 * sizeof(v4f), "holds the sums afterwards");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long m0 = (long)blockIdx.y * 16 * MT;
+    v4i* own = lds[wave];
+    // a lane loads piece lane % 8 of rows lane / 8 and lane / 8 + 8 of w (0) and of MT blocks of x (rows that
+    // are not there repeat the last one: their results are not stored)
+    const int piece = lane & 7;
+    const uint8_t* from[MT + 1][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = 8 * i + (lane >> 3), n = blockIdx.x * 16 + r;
+        from[0][i] = g.w + (long)(n < g.N ? n : g.N - 1) * g.K + 16 * piece;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const long m = m0 + 16 * t + r;
+            from[t + 1][i] = g.x + (m < g.M ? m : g.M - 1) * g.K + 16 * piece;
+        }
+    }
+    v4f acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    v4i in[MT + 1][2];
+    const auto load = [&](int k0) {
+        if (k0 + SLICE <= g.K) {
+#pragma unroll
+            for (int t = 0; t <= MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) in[t][i] = reinterpret_cast<const AnyPiece*>(from[t][i] + k0)->v;
+        } else {
+#pragma unroll
+            for (int t = 0; t <= MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) in[t][i] = load_piece(from[t][i] - 16 * piece, k0 + 16 * piece, g.K);
+        }
+    };
+    const auto between = [] {                        // the wavefront's accesses to LDS stay on their sides
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    const auto operand = [&](int t) {
+        const v4i p = own[t * ROWS16 + piece_at(lane & 15, lane >> 4)], q = own[t * ROWS16 + piece_at(lane & 15, (lane >> 4) + 4)];
+        return v8i{p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+    };
+    int k0 = wave * SLICE;
+    if (k0 < g.K) load(k0);
+    for (; k0 < g.K; k0 += FEW_WAVES * SLICE) {
+#pragma unroll
+        for (int t = 0; t <= MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) own[t * ROWS16 + piece_at(8 * i + (lane >> 3), piece)] = in[t][i];
+        between();
+        if (k0 + FEW_WAVES * SLICE < g.K) load(k0 + FEW_WAVES * SLICE);
+        const v8i a = operand(0);
+        if constexpr (WIDENED<T>) {
+            v8h ah[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ah[i] = widen8(a, i);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const v8i b = operand(t + 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[i], widen8(b, i), acc[t], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, operand(t + 1), acc[t], 0, 0, 0, 0, 0, 0);
+        }
+        between();
+    }
+    __syncthreads();
+    v4f(*sums)[MT][64] = reinterpret_cast<v4f(*)[MT][64]>(lds);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int t = wave; t < MT; t += FEW_WAVES) {
+        v4f total = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < FEW_WAVES; ++v) total += sums[v][t][lane];
+        const float four[4] = {total.x, total.y, total.z, total.w};
+        store4<T>(g, m0 + 16 * t + (lane & 15), blockIdx.x * 16 + 4 * (lane >> 4), four);
+    }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
@@ -367,7 +409,8 @@ __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
 // operands of the next half are read into registers of their own.  When the second half of one double
 // slice has been read by everybody, the double slice after next is asked for into its place: it has two
 // steps (2048 cycles) to arrive.  One barrier per double slice, before its first half is read: a wavefront
-// waits there until its own pieces have arrived, and behind the barrier everybody's have. 
+// waits there until its own pieces have arrived, and behind the barrier everybody's have.  Double slices go
+// in pairs, one for each buffer; behind an odd number of them comes one of zeros.
 //
 // Rows that are not there repeat the last one (their results are not stored).  Where k ends inside the
 // last slice, pieces behind the end repeat the row's last piece and are replaced by zero on their way
@@ -542,13 +585,13 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
         const long bn = (N + BIG - 1) / BIG, bm = (M + BIG - 1) / BIG;
         // Which form, by sizes (bfloat16 results, us):
         // - up to 64 rows, k < 16, or fewer than 64 tiles of 128 x 128 (a quarter of the card's units): few rows.
-        //   512^3 4.1 against 8.3 in tiles, 128 x 4096 x 4096 21 against 34; at 64 tiles (1024^3) 12 each,
-        //   256 x 4096 x 4096 39 against 34.
-        // - tiles of 256 x 256 that fill the card's units to seven eighths in every round, k long enough to
-        //   hide that such a tile neither starts nor ends under another one's work, and rows of whole
-        //   16-byte pieces: large tiles.  4096 x 4096 (256 of them) with k = 4096: 67 against 84 in tiles of
-        //   128; k = 1536, 16384 rows: 128 each; k = 1024: 100 against 92.  196 of them (3328 x 3328): 63
-        //   against 59.
+        //   512^3 3.4 against 6.3 in tiles, 128 x 4096 x 4096 12.6 against 26; at 64 tiles 1024^3 takes 11.9
+        //   against 9.5, 256 x 4096 x 4096 25.5 against 27.
+        // - tiles of 256 x 256 whose results fill five eighths of the card's units in every round, k long
+        //   enough to hide that such a tile neither starts nor ends under another one's work, and rows of
+        //   whole 16-byte pieces: large tiles.  16384 x 4096: k = 1280 94 against 101 in tiles of 128,
+        //   k = 1024 83 against 87, k = 768 75 against 69.  3328 x 3328 x 4096 (66 % of the units) 49 against
+        //   54, 4352 x 4096 x 4096 (53 %) 92 against 84.
         // (blockIdx.y is 16 bits: rows beyond go in further launches)
         const auto in_parts = [&](long rows_each, auto&& launch) {
             for (long first = 0; first < M; first += 65535 * rows_each) {
@@ -576,7 +619,7 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
         }
         if constexpr (!WIDENED<T>) {
             const long units = device_compute_units(), rounds = (bn * bm + units - 1) / units;
-            if (bn * bm * 8 >= rounds * units * 7 && K >= 1536 && K % 16 == 0 && aligned16(x) && aligned16(w)) {
+            if (M * N * 8 >= rounds * units * (5 * BIG * BIG) && K >= 1024 && K % 16 == 0 && aligned16(x) && aligned16(w)) {
                 const unsigned blocks = (unsigned)((bn * bm + 7) / 8 * 8);
                 linear_big_kernel<T><<<dim3(blocks), 256, 0, s>>>(g, (int)bn, (int)bm);
                 return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;

@@ -87,7 +87,8 @@ def test_whole_numbers_are_exact():
 
 
 @pytest.mark.parametrize("M,N,K", [(4096, 4096, 1536), (4090, 3841, 1552), (4097, 7700, 1600), (3841, 4000, 1648), (16000, 1024, 2000),
-                                   (4000, 4000, 1679), (1300, 1300, 640)])
+                                   (4000, 4000, 1679), (1300, 1300, 640), (8100, 4090, 1040), (4096, 4096, 1152),
+                                   (65, 300, 8200), (200, 130, 127), (256, 1000, 1025)])
 def test_large_tiles(M, N, K):
     """Enough 256 x 256 tiles for the large form, ragged in rows, columns and k; NaN behind the rows."""
     import kalman_vae_amd as kv
@@ -100,11 +101,13 @@ def test_large_tiles(M, N, K):
     y = kv.linear_8bit(pads[0], sx, pads[1], sw, bias=bias, dtype=torch.float16)
     rows = torch.cat([torch.arange(0, M, 37), torch.arange(M - 3, M)]).cuda()
     check(y[rows], x[rows], sx[rows], w, sw, bias)
-    # whole numbers of few bits: exact sums (below 2048 and in steps of one)
+    # whole numbers of few bits: exact sums, rounded once to half (a and b draw the same numbers, so row i of one
+    # is row i of the other for i up to their sizes and their product is a sum of squares, two thirds of K: for long
+    # rows beyond 2048, up to which half holds every whole number)
     a, b = (torch.randint(-1, 2, t.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(7)) for t in (x, w))
     one = lambda n: torch.ones(n, device="cuda")  # noqa: E731
     y = kv.linear_8bit(a.float().to(torch.float8_e4m3fn), one(M), b.float().to(torch.float8_e4m3fn), one(N), dtype=torch.float16)
-    assert torch.equal(y.float(), a.float() @ b.float().t().contiguous())
+    assert torch.equal(y, (a.float() @ b.float().t().contiguous()).half())
 
 
 def test_layouts():
