@@ -19,12 +19,11 @@
 // 256 x 256, fed from memory straight into LDS, for large products.
 //
 // Measured (bfloat16 results): 1 x 6144 x 2048 4.3 us (2.9 TB/s), 64 x 4096 x 4096 6.8 us, 262144 x 384 x 128
-// 51 us (4.6 TB/s, memory's rate), 4096^3 58 us, 16384 x 4096 x 4096 220 us = 2.5 PFLOP/s, where the library's
+// 48 us (4.9 TB/s, memory's rate), 4096^3 58 us, 16384 x 4096 x 4096 230 us = 2.4 PFLOP/s, where the library's
 // product of 8-bit operands takes 224 us, and 8192^3 430 us = 2.6.  A loop of nothing but these instructions
 // reaches 3.4 to 4 on random bytes (the clock comes down).  Each round of large tiles spends some 12 us
 // outside its loop (first requests, results); workgroups that stay and ask for the next tile's start before
-// they write the last one's results were no faster (227 to 248 us), nor was a step that warms the second
-// cache two slices ahead (224 us).
+// they write the last one's results were no faster (227 to 248 us).
 #include "narrow_types.h"
 
 #include "device_info.h"
@@ -117,10 +116,11 @@ struct Factors {
 template <int ROWS>
 __device__ __forceinline__ void load_factors(const LinearArgs& g, long m0, int n0, Factors<ROWS>& f) {
     const int i = threadIdx.x;
-    if (i < ROWS) {
-        f.sx[i] = m0 + i < g.M ? g.sx[m0 + i] : 0.f;
-        f.sw[i] = n0 + i < g.N ? g.sw[n0 + i] : 0.f;
-        f.bias[i] = g.bias && n0 + i < g.N ? g.bias[n0 + i] : 0.f;
+    if (i < ROWS) {                                  // (those of rows that are not there are not used)
+        const long m = m0 + i < g.M ? m0 + i : g.M - 1;
+        const int n = n0 + i < g.N ? n0 + i : g.N - 1;
+        const float sx = g.sx[m], sw = g.sw[n], bias = g.bias ? g.bias[n] : 0.f;
+        f.sx[i] = sx, f.sw[i] = sw, f.bias[i] = bias;
     }
 }
 
@@ -410,7 +410,9 @@ __global__ void __launch_bounds__(256, 3) linear_tile_kernel(LinearArgs g) {
 // slice has been read by everybody, the double slice after next is asked for into its place: it has two
 // steps (2048 cycles) to arrive.  One barrier per double slice, before its first half is read: a wavefront
 // waits there until its own pieces have arrived, and behind the barrier everybody's have.  Double slices go
-// in pairs, one for each buffer; behind an odd number of them comes one of zeros.
+// in pairs, one for each buffer; behind an odd number of them comes one of zeros.  Two steps hide the way from
+// the die's cache but not the one from memory, so a step also touches the lines of the double slice after
+// that, shared out among the tiles of a die (inputs that were not used just before: 250 -> 230 us).
 //
 // Rows that are not there repeat the last one (their results are not stored).  Where k ends inside the
 // last slice, pieces behind the end repeat the row's last piece and are replaced by zero on their way
@@ -427,6 +429,7 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
     // asked for: 16384 x 4096 x 4096 264 us).
     __shared__ v4i buffer0[2 * OPERAND], buffer1[2 * OPERAND];
     __shared__ Factors<BIG> factors;
+    __shared__ unsigned unread[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go round the eight dies (blockIdx % 8): each die gets a run of neighbouring tiles, in
     // groups of eight rows of tiles, so that its cache serves the tiles that run together.
@@ -465,6 +468,17 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
                 (const __attribute__((address_space(1))) void*)(wb + (w_row[i] + k)),
                 (__attribute__((address_space(3))) void*)(at + OPERAND + 256 * i), 16, 0, 0);
         }
+    };
+    // One word of a cache line of double slice d, so that it is in the die's cache when the slice is asked for.
+    // The tiles that run together on a die lie four in a row and eight in a column, so each touches a quarter
+    // of its rows of x and an eighth of its rows of w, and the others theirs of the same rows.
+    const int xr = 64 * (rest / rows & 3) + 16 * wave + (lane & 15), wr = 32 * (rest % rows & 7) + 8 * wave + (lane & 7);
+    const uint8_t* line = lane < 16 ? xb + (xr < rows_x ? xr : rows_x - 1) * g.K : wb + (wr < rows_w ? wr : rows_w - 1) * g.K;
+    const auto warm = [&](int d) {
+        __builtin_amdgcn_sched_barrier(0);           // (behind what was asked for before: see arrive)
+        const int at = BIG_SLICE * d < g.K - 16 ? BIG_SLICE * d : g.K - 16;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(line + at),
+                                         (__attribute__((address_space(3))) void*)unread, 4, 0, 0);
     };
     struct Operands {
         v8i a[4], b[4];
@@ -514,10 +528,11 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
         if (!requests) __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    // everything asked for has arrived, for everybody, and everybody's reads are done
-    const auto arrive = [] {
+    // Everything asked for has arrived, for everybody, and everybody's reads are done.  BUT: the last requests
+    // that need not have arrived (they come in order).
+    const auto arrive = [](auto but) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);          // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_waitcnt(0x0070 | decltype(but)::value);   // vmcnt(BUT) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
@@ -533,6 +548,8 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
             }
     };
     const int doubles = (g.K + BIG_SLICE - 1) / BIG_SLICE;
+    constexpr std::integral_constant<int, 0> b0{};
+    constexpr std::integral_constant<int, 1> b1{};
     Operands first, second;
     const auto step = [&](auto b, int d) {
         constexpr std::integral_constant<int, 1 - decltype(b)::value> other{};
@@ -542,21 +559,21 @@ __global__ void __launch_bounds__(256, 1) linear_big_kernel(LinearArgs g, int ti
         multiply(first);
         interleave(false);
         if (ends) cut(d, 1, second);
-        arrive();                                    // d + 1 is there, nobody reads d any more
+        arrive(b1);                                  // d + 1 is there, nobody reads d any more
         fetch(b, d + 2);                             // (behind the end of k: not used)
         read(other, 0, first);
         multiply(second);
         interleave(true);
+        warm(d + 3);
     };
-    constexpr std::integral_constant<int, 0> b0{};
-    constexpr std::integral_constant<int, 1> b1{};
     fetch(b0, 0);
     load_factors(g, m0, n0, factors);
-    arrive();
+    arrive(b0);
     fetch(b1, 1);
+    warm(2);
     read(b0, 0, first);
     for (int d = 0; d < doubles; d += 2) step(b0, d), step(b1, d + 1);
-    arrive();                                        // nothing is under way, the operands' LDS is free
+    arrive(b0);                                      // nothing is under way, the operands' LDS is free
     // (a wavefront's 32 KB lie in one of the buffers)
     char* region = reinterpret_cast<char*>(wave < 2 ? buffer0 : buffer1) + (wave & 1) * (128 * 128 * (int)sizeof(T));
     write_rows<T, 128, 4>(g, factors, region, m0, n0, wm, wn, lane,
