@@ -745,9 +745,9 @@ int kvae_gated_scan_step(int64_t B, int64_t H, int dtype, int gated, const void 
  *   the inverse root (the backward call needs it).
  * quantized: y (rows,D) in e4m3 bytes and scale (rows) float with y = q scale:
  *   scale = max(max |y| / 448, 2^-126), to the nearest; a NaN stays one and does not enter the scale.
- * backward: r is formed again from x and residual (or pass the stored sum as x and residual = NULL);
- *   writes dx = the gradient w.r.t. x and w.r.t. residual alike, with dsum (or NULL), the gradient
- *   that reaches sum, added; and dweight.  partial: kvae_rms_norm_backward_parts(rows) x D floats.
+ * backward: r is formed again from x and residual (a stored sum may be passed as x, with residual =
+ *   NULL, where its rounding does not matter); writes dx = the gradient w.r.t. x and w.r.t. residual
+ *   alike, with dsum (or NULL), the gradient that reaches sum, added; and dweight.  partial: kvae_rms_norm_backward_parts(rows) x D floats.
  * kvae_quantize_rows: the same e4m3 form of the rows of x as they are.                        */
 #define KVAE_NORM_MAX_WIDTH 16384
 typedef struct {

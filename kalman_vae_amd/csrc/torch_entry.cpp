@@ -244,10 +244,10 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
                                  const OptTensor& residual, double eps) {
         auto out = norm_forward(x, weight, residual, eps, true);
-        // The backward pass forms the unrounded sum again from x and residual where the gradient of
-        // a float weight would show the 16-bit sum's rounding; elsewhere the stored sum serves (one
-        // tensor less to keep and to read).
-        const bool again = residual && x.scalar_type() != weight.scalar_type();
+        // The backward pass reads the stored sum if that is the sum itself (float).  A 16-bit one is rounded,
+        // which is as much as the weight's gradient is rounded by and would add to it; there the sum is
+        // formed again from x and residual (8192 x 4096 bfloat16 75 us instead of 51).
+        const bool again = residual && x.scalar_type() != at::kFloat;
         ctx->save_for_backward({residual && !again ? out[1] : x, again ? *residual : Tensor(), weight, out[2]});
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["residual"] = residual.has_value();

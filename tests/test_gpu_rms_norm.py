@@ -70,17 +70,16 @@ def test_forward_and_backward(D, dtype, wide_weight, with_residual):
     check(y, want, k * want.abs(), "y")
     if with_residual:
         check(total, r, UNIT * r.abs(), "sum")
-    # gradients; where the stored 16-bit sum serves, r is off by its rounding
-    off = half_step(dtype) if with_residual and dtype == w.dtype else 0.0
+    # gradients (of the unrounded sum whatever the types)
     n, d = r * s, dy.double() * w.double()
     along, size = (d * n).mean(1, keepdim=True), (d * n).abs().mean(1, keepdim=True)
     grad = s * (d - n * along) + (dsum.double() if dsum is not None else 0.0)
-    err = (k + 2 * off) * s * (d.abs() + 2 * n.abs() * size) + UNIT * grad.abs()
+    err = k * s * (d.abs() + 2 * n.abs() * size) + UNIT * grad.abs()
     check(dx, grad, err, "dx")
     if with_residual:
         assert torch.equal(dx, dres)
     terms = dy.double() * n
-    check(dw, terms.sum(0), (k + rows * UNIT + off) * terms.abs().sum(0), "dw")
+    check(dw, terms.sum(0), (k + rows * UNIT) * terms.abs().sum(0), "dw")
     again = run(x, residual, w, dy, dsum)
     assert all(a is None or torch.equal(a, b) for a, b in zip((y, total, dx, dw, dres), again))
 
