@@ -89,8 +89,19 @@ void* address(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : n
 Tensor rows_dense(const Tensor& t) {
     return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
 }
-// (rows, D) with last-axis stride 1; copies only when the leading axes do not merge
-Tensor as_rows(const Tensor& t, int64_t D) { return rows_dense(t).reshape({-1, D}); }
+// A tensor as rows of D with last-axis stride 1, copied only when its leading axes do not merge.  (A view
+// would do for all of them, at a microsecond each.)
+struct Rows {
+    Rows() = default;
+    Rows(const Tensor& t, int64_t D) : held(t), stride(D) {
+        if (!t.is_contiguous()) held = rows_dense(t).reshape({-1, D}), stride = held.stride(0);
+        at = held.data_ptr();
+    }
+    Tensor held;
+    void* at = nullptr;
+    int64_t stride = 0;
+};
+Rows rows_of(const OptTensor& t, int64_t D) { return t && t->defined() ? Rows(*t, D) : Rows(); }
 
 // A tensor that a kernel has written in place: autograd's saved copies of it are stale, and whoever
 // keeps something made from it can see so.
@@ -216,12 +227,12 @@ Tensor gated_scan_step(const Tensor& u_in, const Tensor& state, const OptTensor&
 }
 
 // -- norm -------------------------------------------------------------------------------------
-kvae_rms_norm norm_struct(const Tensor& x2, const Tensor& r2, const Tensor& weight, double eps) {
+kvae_rms_norm norm_struct(const Tensor& x, const Rows& rows, const Rows& residual, const Tensor& weight, double eps) {
     kvae_rms_norm d{};
-    d.rows = x2.size(0), d.D = x2.size(1);
-    d.dtype = dtype_code(x2.scalar_type()), d.weight_dtype = dtype_code(weight.scalar_type());
-    d.x = x2.data_ptr(), d.x_stride = x2.stride(0);
-    if (r2.defined()) d.residual = r2.data_ptr(), d.residual_stride = r2.stride(0);
+    d.D = x.size(-1), d.rows = x.numel() / d.D;
+    d.dtype = dtype_code(x.scalar_type()), d.weight_dtype = dtype_code(weight.scalar_type());
+    d.x = rows.at, d.x_stride = rows.stride;
+    d.residual = residual.at, d.residual_stride = residual.stride;
     d.weight = weight.data_ptr(), d.eps = (float)eps;
     return d;
 }
@@ -230,11 +241,11 @@ std::array<Tensor, 3> norm_forward(const Tensor& x, const Tensor& weight, const 
                                    bool keep) {
     const On on(x);
     const int64_t D = x.size(-1);
-    const Tensor x2 = as_rows(x, D), r2 = residual ? as_rows(*residual, D) : Tensor();
+    const Rows rows(x, D), res = rows_of(residual, D);
     std::array<Tensor, 3> out = {empty(x.sizes(), x), Tensor(), Tensor()};
     if (residual) out[1] = empty(x.sizes(), x);
-    if (keep) out[2] = empty({x2.size(0)}, x, at::kFloat);
-    kvae_rms_norm d = norm_struct(x2, r2, weight, eps);
+    if (keep) out[2] = empty({x.numel() / D}, x, at::kFloat);
+    kvae_rms_norm d = norm_struct(x, rows, res, weight, eps);
     d.y = out[0].data_ptr(), d.sum = address(out[1]), d.rstd = address(out[2]);
     check(lib.norm_forward(&d, on.stream));
     return out;
@@ -249,8 +260,6 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
         // formed again from x and residual (8192 x 4096 bfloat16 75 us instead of 51).
         const bool again = residual && x.scalar_type() != at::kFloat;
         ctx->save_for_backward({residual && !again ? out[1] : x, again ? *residual : Tensor(), weight, out[2]});
-        ctx->saved_data["eps"] = eps;
-        ctx->saved_data["residual"] = residual.has_value();
         ctx->set_materialize_grads(false);
         return residual ? variable_list{out[0], out[1]} : variable_list{out[0]};
     }
@@ -263,18 +272,18 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
             const On on(x);
             const int64_t D = x.size(-1);
             const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(x.sizes(), x.options());
-            const Tensor dsum = grads.size() > 1 ? grads[1] : Tensor();
-            const Tensor x2 = as_rows(x, D), r2 = residual.defined() ? as_rows(residual, D) : Tensor();
-            const Tensor dy2 = as_rows(dy, D), ds2 = dsum.defined() ? as_rows(dsum, D) : Tensor();
+            const bool two = grads.size() > 1;       // (with a residual)
+            const Rows rows(x, D), res = rows_of(residual, D), dy_rows(dy, D),
+                       dsum = two ? rows_of(grads[1], D) : Rows();
             out[0] = empty(x.sizes(), x);
             out[1] = empty({D}, weight);
-            const Tensor partial = empty({lib.norm_parts(x2.size(0)), D}, x, at::kFloat);
-            kvae_rms_norm d = norm_struct(x2, r2, weight, ctx->saved_data["eps"].toDouble());
-            d.rstd = rstd.data_ptr(), d.dy = dy2.data_ptr(), d.dy_stride = dy2.stride(0);
-            if (ds2.defined()) d.dsum = ds2.data_ptr(), d.dsum_stride = ds2.stride(0);
+            kvae_rms_norm d = norm_struct(x, rows, res, weight, 0.0);
+            const Tensor partial = empty({lib.norm_parts(d.rows), D}, x, at::kFloat);
+            d.rstd = rstd.data_ptr(), d.dy = dy_rows.at, d.dy_stride = dy_rows.stride;
+            d.dsum = dsum.at, d.dsum_stride = dsum.stride;
             d.dx = out[0].data_ptr(), d.partial = partial.data_ptr(), d.dweight = out[1].data_ptr();
             check(lib.norm_backward(&d, on.stream));
-            if (ctx->saved_data["residual"].toBool()) out[2] = out[0];
+            if (two) out[2] = out[0];
         }
         grads.insert(grads.end(), {x, residual, weight});
         return once_differentiable(std::move(out), grads);
@@ -297,13 +306,13 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_quantized(const Tensor& x, const 
                                                          const OptTensor& residual, double eps) {
     const On on(x);
     const int64_t D = x.size(-1);
-    const Tensor weight = weight_in.contiguous(), x2 = as_rows(x, D);
-    const Tensor r2 = residual ? as_rows(*residual, D) : Tensor();
+    const Tensor weight = weight_in.contiguous();
+    const Rows rows(x, D), res = rows_of(residual, D);
     Tensor q = empty(x.sizes(), x, at::kFloat8_e4m3fn);
     Tensor scale = empty(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
     OptTensor sum;
     if (residual) sum = empty(x.sizes(), x);
-    kvae_rms_norm d = norm_struct(x2, r2, weight, eps);
+    kvae_rms_norm d = norm_struct(x, rows, res, weight, eps);
     d.y = q.data_ptr(), d.scale = scale.data_ptr(), d.sum = address(sum);
     check(lib.norm_quantized(&d, on.stream));
     return {q, scale, sum};
@@ -311,11 +320,12 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_quantized(const Tensor& x, const 
 
 std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
     const On on(x);
-    const Tensor x2 = as_rows(x, x.size(-1));
+    const int64_t D = x.size(-1);
+    const Rows rows(x, D);
     Tensor q = empty(x.sizes(), x, at::kFloat8_e4m3fn);
     Tensor scale = empty(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
-    check(lib.quantize_rows(x2.size(0), x2.size(1), dtype_code(x.scalar_type()), x2.data_ptr(), x2.stride(0),
-                            q.data_ptr(), scale.data_ptr(), on.stream));
+    check(lib.quantize_rows(x.numel() / D, D, dtype_code(x.scalar_type()), rows.at, rows.stride, q.data_ptr(),
+                            scale.data_ptr(), on.stream));
     return {q, scale};
 }
 
