@@ -13,12 +13,12 @@
 // first operand's place: then a lane's results are four neighbouring n of one row m, which go out
 // as one wide store, and the matrix instruction's k order does not matter as both sides share it.
 //
-// Three forms.  Few rows: reading w once is the work; a workgroup takes 16 rows of w and up to 64 of x, its
-// wavefronts share out k and add up through LDS.  Tiles of 128 x 128 staged through registers and LDS, the
+// Three forms.  Few rows: reading w once is the work; a workgroup takes 16 rows of w (64 when there are enough
+// of them) and up to 64 of x, its wavefronts share out k and add up through LDS.  Tiles of 128 x 128 staged through registers and LDS, the
 // next slice of k on its way while the present one is multiplied, three workgroups to a unit.  Large tiles of
 // 256 x 256, fed from memory straight into LDS, for large products.
 //
-// Measured (bfloat16 results): 1 x 6144 x 2048 4.3 us (2.9 TB/s), 64 x 4096 x 4096 6.8 us, 262144 x 384 x 128
+// Measured (bfloat16 results): 1 x 6144 x 2048 4.3 us (2.9 TB/s), 64 x 4096 x 4096 7 us, 1024^3 6.1, 256 x 4096 x 4096 12, 262144 x 384 x 128
 // 48 us (4.9 TB/s, memory's rate), 4096^3 58 us, 16384 x 4096 x 4096 230 us = 2.4 PFLOP/s, where the library's
 // product of 8-bit operands takes 224 us, and 8192^3 430 us = 2.6.  A loop of nothing but these instructions
 // reaches 3.4 to 4 on random bytes (the clock comes down).  Each round of large tiles spends some 12 us
@@ -59,12 +59,8 @@ __device__ __forceinline__ v4i shift_down(const v4i& r, int bytes) {
     return v4i{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 
-// 16 bytes of a row of K from byte k on, at any address; bytes at K and beyond are zero.  A piece that
-// ends behind the row is the row's last 16 bytes shifted down.
-__device__ __forceinline__ v4i load_piece(const uint8_t* row, int k, int K) {
-    if (k + 16 <= K) return reinterpret_cast<const AnyPiece*>(row + k)->v;
-    if (k >= K) return v4i{0, 0, 0, 0};
-    if (K >= 16) return shift_down(reinterpret_cast<const AnyPiece*>(row + K - 16)->v, k + 16 - K);
+// 16 bytes of a row of K < 16 from byte k on; bytes at K and beyond are zero
+__device__ __forceinline__ v4i first_bytes(const uint8_t* row, int k, int K) {
     unsigned long lo = 0, hi = 0;
 #pragma unroll 1
     for (int i = 0; k + i < K; ++i) (i < 8 ? lo : hi) |= (unsigned long)row[k + i] << (8 * (i & 7));
@@ -199,47 +195,60 @@ __device__ __forceinline__ int row_key(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int piece_at(int r, int c) { return r * (SLICE / 16) + (c ^ row_key(r)); }
 
 constexpr int FEW_WAVES = 8;
-// Rows of x: blockIdx.y * 16 MT ..., rows of w: blockIdx.x * 16 ...  The wavefronts share out k in slices of
+// Rows of x: blockIdx.y * 16 MT ..., rows of w: blockIdx.x * 16 NT ...  The wavefronts share out k in slices of
 // 128 bytes.  The matrix instruction wants 16 rows side by side in 16 neighbouring lanes; loaded like that,
 // every lane would be in another cache line (57 cycles of the address unit for an instruction of 1 KB).
 // So eight lanes load a line, and the rows change lanes in LDS of the wavefront's own.
-template <typename T, int MT>
+template <typename T, int MT, int NT>
 __global__ void __launch_bounds__(64 * FEW_WAVES) linear_few_rows_kernel(LinearArgs g) {
     constexpr int ROWS16 = 16 * SLICE / 16;          // pieces of 16 rows
-    __shared__ v4i lds[FEW_WAVES][(MT + 1) * ROWS16];
-    static_assert(sizeof(lds) >= FEW_WAVES * MT * 64 * sizeof(v4f), "holds the sums afterwards");
+    __shared__ v4i lds[FEW_WAVES][(MT + NT) * ROWS16];
+    static_assert(sizeof(lds) >= FEW_WAVES * MT * NT * 64 * sizeof(v4f), "holds the sums afterwards");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long m0 = (long)blockIdx.y * 16 * MT;
+    const int n0 = blockIdx.x * 16 * NT;
     v4i* own = lds[wave];
-    // a lane loads piece lane % 8 of rows lane / 8 and lane / 8 + 8 of w (0) and of MT blocks of x (rows that
-    // are not there repeat the last one: their results are not stored)
+    // a lane loads piece lane % 8 of rows lane / 8 and lane / 8 + 8 of NT blocks of w and of MT blocks of x
+    // (rows that are not there repeat the last one: their results are not stored)
     const int piece = lane & 7;
-    const uint8_t* from[MT + 1][2];
+    const uint8_t *xb = g.x + m0 * g.K, *wb = g.w + (long)n0 * g.K;
+    const unsigned row0 = (unsigned)(lane >> 3) * (unsigned)g.K;     // byte offsets from the first rows
+    const unsigned x_end = (unsigned)(g.M - m0 < 16 * MT ? g.M - m0 - 1 : 16 * MT - 1) * (unsigned)g.K;
+    const unsigned w_end = (unsigned)(g.N - n0 < 16 * NT ? g.N - n0 - 1 : 16 * NT - 1) * (unsigned)g.K;
+    const auto from = [&](int t, int i) {
+        const unsigned row = row0 + (unsigned)(16 * (t < NT ? t : t - NT) + 8 * i) * (unsigned)g.K;
+        return t < NT ? wb + (row < w_end ? row : w_end) : xb + (row < x_end ? row : x_end);
+    };
+    v4f acc[MT][NT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = 8 * i + (lane >> 3), n = blockIdx.x * 16 + r;
-        from[0][i] = g.w + (long)(n < g.N ? n : g.N - 1) * g.K + 16 * piece;
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const long m = m0 + 16 * t + r;
-            from[t + 1][i] = g.x + (m < g.M ? m : g.M - 1) * g.K + 16 * piece;
-        }
-    }
-    v4f acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-    v4i in[MT + 1][2];
+        for (int u = 0; u < NT; ++u) acc[t][u] = v4f{0.f, 0.f, 0.f, 0.f};
+    v4i in[NT + MT][2];
     const auto load = [&](int k0) {
         if (k0 + SLICE <= g.K) {
 #pragma unroll
-            for (int t = 0; t <= MT; ++t)
+            for (int t = 0; t < NT + MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) in[t][i] = reinterpret_cast<const AnyPiece*>(from[t][i] + k0)->v;
+                for (int i = 0; i < 2; ++i) in[t][i] = reinterpret_cast<const AnyPiece*>(from(t, i) + (k0 + 16 * piece))->v;
+        } else if (NT > 1 || g.K >= 16) {            // (NT > 1 is for K >= 16)
+            // pieces that end behind the row are its last 16 bytes shifted down
+            const int k = k0 + 16 * piece, at = k < g.K - 16 ? k : g.K - 16;
+#pragma unroll
+            for (int t = 0; t < NT + MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) in[t][i] = reinterpret_cast<const AnyPiece*>(from(t, i) + at)->v;
+            if (k > at) {
+#pragma unroll
+                for (int t = 0; t < NT + MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) in[t][i] = shift_down(in[t][i], k - at);
+            }
         } else {
 #pragma unroll
-            for (int t = 0; t <= MT; ++t)
+            for (int t = 0; t < NT + MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) in[t][i] = load_piece(from[t][i] - 16 * piece, k0 + 16 * piece, g.K);
+                for (int i = 0; i < 2; ++i) in[t][i] = first_bytes(from(t, i), k0 + 16 * piece, g.K);
         }
     };
     const auto between = [] {                        // the wavefront's accesses to LDS stay on their sides
@@ -255,41 +264,56 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) linear_few_rows_kernel(LinearA
     if (k0 < g.K) load(k0);
     for (; k0 < g.K; k0 += FEW_WAVES * SLICE) {
 #pragma unroll
-        for (int t = 0; t <= MT; ++t)
+        for (int t = 0; t < NT + MT; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) own[t * ROWS16 + piece_at(8 * i + (lane >> 3), piece)] = in[t][i];
         between();
         if (k0 + FEW_WAVES * SLICE < g.K) load(k0 + FEW_WAVES * SLICE);
-        const v8i a = operand(0);
+        v8i a[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) a[u] = operand(u);
         if constexpr (WIDENED<T>) {
-            v8h ah[4];
+            // (quarter by quarter, so that the widened operands of one only are in registers)
+            v8i b[MT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ah[i] = widen8(a, i);
+            for (int t = 0; t < MT; ++t) b[t] = operand(NT + t);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const v8i b = operand(t + 1);
+            for (int i = 0; i < 4; ++i) {
+                v8h ah[NT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[i], widen8(b, i), acc[t], 0, 0, 0);
+                for (int u = 0; u < NT; ++u) ah[u] = widen8(a[u], i);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const v8h bh = widen8(b[t], i);
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+                        acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[u], bh, acc[t][u], 0, 0, 0);
+                }
             }
         } else {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, operand(t + 1), acc[t], 0, 0, 0, 0, 0, 0);
+            for (int t = 0; t < MT; ++t) {
+                const v8i b = operand(NT + t);
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+                    acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[u], b, acc[t][u], 0, 0, 0, 0, 0, 0);
+            }
         }
         between();
     }
     __syncthreads();
-    v4f(*sums)[MT][64] = reinterpret_cast<v4f(*)[MT][64]>(lds);
+    v4f(*sums)[MT * NT][64] = reinterpret_cast<v4f(*)[MT * NT][64]>(lds);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) sums[wave][t * NT + u][lane] = acc[t][u];
     __syncthreads();
-    for (int t = wave; t < MT; t += FEW_WAVES) {
+    for (int t = wave; t < MT * NT; t += FEW_WAVES) {
         v4f total = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < FEW_WAVES; ++v) total += sums[v][t][lane];
         const float four[4] = {total.x, total.y, total.z, total.w};
-        store4<T>(g, m0 + 16 * t + (lane & 15), blockIdx.x * 16 + 4 * (lane >> 4), four);
+        store4<T>(g, m0 + 16 * (t / NT) + (lane & 15), n0 + 16 * (t % NT) + 4 * (lane >> 4), four);
     }
 }
 
@@ -598,12 +622,15 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
                            static_cast<const uint8_t*>(w), static_cast<const float*>(x_scale),
                            static_cast<const float*>(w_scale), static_cast<const float*>(bias), y};
         const hipStream_t s = static_cast<hipStream_t>(stream);
-        const long tn = (N + TILE - 1) / TILE, tm = (M + TILE - 1) / TILE;
+        const long tn = (N + TILE - 1) / TILE;
         const long bn = (N + BIG - 1) / BIG, bm = (M + BIG - 1) / BIG;
         // Which form, by sizes (bfloat16 results, us):
-        // - up to 64 rows, k < 16, or fewer than 64 tiles of 128 x 128 (a quarter of the card's units): few rows.
-        //   512^3 3.4 against 6.3 in tiles, 128 x 4096 x 4096 12.6 against 26; at 64 tiles 1024^3 takes 11.9
-        //   against 9.5, 256 x 4096 x 4096 25.5 against 27.
+        // - a few rows: blocks of 16 columns by all rows up to 64, k shared out; 64 x 4096 x 4096 7 against 10 in
+        //   blocks of 64 x 64 and 27 in tiles of 128, 512^3 3.9 against 6.1 and 6.2.  Also where k < 16.
+        // - 64 x 64 blocks, k shared out, when there are 96 to 256 of them, one for a unit of the card (up to two
+        //   if k is long): 128 x 4096 x 4096 10 against 13 in 16 columns and 27 in tiles, 256 x 4096 x 4096 12
+        //   against 23 and 27, 1024^3 6.1 against 10 and 9.4; 512 of them with k = 4096 21 against 29 in tiles,
+        //   with k = 1024 11.1 against 10.
         // - tiles of 256 x 256 whose results fill five eighths of the card's units in every round, k long
         //   enough to hide that such a tile neither starts nor ends under another one's work, and rows of
         //   whole 16-byte pieces: large tiles.  16384 x 4096: k = 1280 94 against 101 in tiles of 128,
@@ -622,17 +649,23 @@ extern "C" int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void* x, 
             }
             return hipGetLastError() == hipSuccess ? KVAE_OK : KVAE_E_LAUNCH;
         };
-        if (M <= 64 || K < 16 || tn * tm < 64) {
-            const unsigned nb = (unsigned)((N + 15) / 16);
-            return in_parts(64, [&](const LinearArgs& h, unsigned count) {
-                if (M <= 16) {
-                    linear_few_rows_kernel<T, 1><<<dim3(nb), 64 * FEW_WAVES, 0, s>>>(h);
-                } else if (M <= 32) {
-                    linear_few_rows_kernel<T, 2><<<dim3(nb), 64 * FEW_WAVES, 0, s>>>(h);
-                } else {
-                    linear_few_rows_kernel<T, 4><<<dim3(nb, count), 64 * FEW_WAVES, 0, s>>>(h);
-                }
-            });
+        const long blocks64 = ((M + 63) / 64) * ((N + 63) / 64);
+        const bool blocks = M > 32 && K >= 16 && blocks64 >= 96 && (blocks64 <= 256 || (blocks64 <= 512 && K >= 2048));
+        if (blocks || M <= 64 || K < 16 || blocks64 < 96) {
+            const auto go = [&](auto mt, auto nt) {
+                constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value;
+                return in_parts(16 * MT, [&](const LinearArgs& h, unsigned count) {
+                    linear_few_rows_kernel<T, MT, NT>
+                        <<<dim3((unsigned)((N + 16 * NT - 1) / (16 * NT)), count), 64 * FEW_WAVES, 0, s>>>(h);
+                });
+            };
+            constexpr std::integral_constant<int, 1> one{};
+            constexpr std::integral_constant<int, 2> two{};
+            constexpr std::integral_constant<int, 4> four{};
+            if (blocks) return go(four, four);
+            if (M <= 16) return go(one, one);
+            if (M <= 32) return go(two, one);
+            return go(four, one);
         }
         if constexpr (!WIDENED<T>) {
             const long units = device_compute_units(), rounds = (bn * bm + units - 1) / units;

@@ -227,7 +227,8 @@ class GatedModel(nn.Module):
     def eight_bit(self, on=True):
         """Lay out (or, with ``on=False``, drop) the 8-bit form of the blocks' projections: 1 byte per
         weight and one float32 scale per output.  Later calls without a gradient use it; a call
-        after the parameters have changed raises until this is called again.  Returns self."""
+        after the parameters have changed raises until this is called again.  Moving or converting the
+        module drops it.  Returns self."""
         self._eight = None
         if on:
             capi.require_gpu(self.norm)

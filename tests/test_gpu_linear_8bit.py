@@ -88,7 +88,8 @@ def test_whole_numbers_are_exact():
 
 @pytest.mark.parametrize("M,N,K", [(4096, 4096, 1536), (4090, 3841, 1552), (4097, 7700, 1600), (3841, 4000, 1648), (16000, 1024, 2000),
                                    (4000, 4000, 1679), (1300, 1300, 640), (8100, 4090, 1040), (4096, 4096, 1152),
-                                   (65, 300, 8200), (200, 130, 127), (256, 1000, 1025)])
+                                   (65, 300, 8200), (200, 130, 127), (256, 1000, 1025), (250, 2500, 1100), (777, 1000, 16), (40, 6200, 17),
+                                   (500, 4000, 2049), (64, 40000, 33)])
 def test_large_tiles(M, N, K):
     """Enough 256 x 256 tiles for the large form, ragged in rows, columns and k; NaN behind the rows."""
     import kalman_vae_amd as kv
