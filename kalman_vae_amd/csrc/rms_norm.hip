@@ -5,7 +5,7 @@
 //   dr = s (w dy - n mean(w dy n)) + g_r with n = r s,  dw = sum over rows of dy n
 //
 // Bound by memory: every input is read once and every output written once.  A row stays in the
-// registers of LPR lanes (16, 64, 256 or 1024: a quarter wavefront for the narrow rows of the weight
+// registers of LPR lanes (16, 64, 256, 512 or 1024: a quarter wavefront for the narrow rows of the weight
 // network up to a whole workgroup of 16 wavefronts), N vectors of 16 bytes per lane, so that the
 // second use of a row (after its sum of squares is known) costs no second read.
 //
@@ -15,7 +15,7 @@
 // fixed order: no atomics, the same bits on every run.
 //
 // Measured, where a large copy moves 5.1 TB/s: with a residual, 81920 x 128 float 30.5 us forward (5.5 TB/s),
-// 28 + 4 us backward; 8192 x 4096 bfloat16 49 us (5.5) and 75 + 5 us; to e4m3, 262144 x 256 bfloat16 89 us
+// 28 + 4 us backward; 8192 x 4096 bfloat16 43 us and 71 + 4 us; to e4m3, 262144 x 256 bfloat16 88 us
 // (5.3).  Few rows are bound by their launches: 2.5 to 4 us for each of the three.
 #include "narrow_types.h"
 
@@ -373,8 +373,11 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(long parts, int 
     }
 }
 
-// Lanes per row and vectors per lane: the fewest lanes whose registers hold the row in at most four
-// vectors each, so that a narrow row does not leave lanes idle and a wide one does not spill.
+// Lanes per row and vectors per lane: the fewest lanes that hold the row in one or two vectors each (beyond
+// 1024 lanes more), so that a narrow row does not leave lanes idle and the backward kernel's four rows of
+// floats leave room for four to six wavefronts to a SIMD.  (Up to four vectors of eight 16-bit elements took
+// 221 registers; backward, bfloat16: 16384 x 2048 101 us against 71, 4096 x 8192 102 against 68, 65536 x 512
+// 105 against 69; forward 45 to 51 against 43 to 45.)
 template <typename T, typename F>
 static int with_shape(int D, F&& f) {
     constexpr int V = 16 / sizeof(T);
@@ -385,11 +388,11 @@ static int with_shape(int D, F&& f) {
         return call(std::integral_constant<int, LPR>{}, std::integral_constant<int, N>{});
     KVAE_NORM_SHAPE(16, 1)
     KVAE_NORM_SHAPE(16, 2)
-    KVAE_NORM_SHAPE(16, 4)
+    KVAE_NORM_SHAPE(64, 1)
     KVAE_NORM_SHAPE(64, 2)
-    KVAE_NORM_SHAPE(64, 4)
-    KVAE_NORM_SHAPE(256, 2)
-    KVAE_NORM_SHAPE(256, 4)
+    KVAE_NORM_SHAPE(256, 1)
+    KVAE_NORM_SHAPE(512, 1)
+    KVAE_NORM_SHAPE(1024, 1)
     KVAE_NORM_SHAPE(1024, 2)
     if constexpr (sizeof(T) == 4) { KVAE_NORM_SHAPE(1024, 4) }   // 16-bit rows end at 1024 x 2
 #undef KVAE_NORM_SHAPE
@@ -447,12 +450,11 @@ static int run_forward(int dtype, const NormArgs& all, hipStream_t stream) {
     });
 }
 
-// Workgroups of the backward kernel = partial rows of dw: four per compute unit fill the card, fewer
-// when there are not eight rows for each (8192 x 4096 bfloat16: 1024 of them 52 us and 6 for their sum,
-// 512 of them 79 and 4, 2048 of them 57 and 12).
+// Workgroups of the backward kernel = partial rows of dw, at most (the buffer's): four per compute unit fill
+// the card, fewer when there are not four rows for each.
 static long norm_parts(long rows) {
     const long most = 4L * device_compute_units();
-    const long want = (rows + 7) / 8;
+    const long want = (rows + 3) / 4;
     return want < most ? want : most;
 }
 
@@ -497,7 +499,12 @@ extern "C" int kvae_rms_norm_backward(const kvae_rms_norm* d, void* stream) {
         using T = decltype(e);
         return with_shape<T>(g.D, [&](auto lpr, auto n) {
             constexpr int LPR = decltype(lpr)::value, N = decltype(n)::value;
-            const long parts = norm_parts(g.rows);
+            // as many as there are rows for, and as fit on the card at once (wide rows take 512 and 1024 threads:
+            // 8192 x 3000 bfloat16 48 us with three of 512 to a unit, 64 with four)
+            constexpr int RPB = norm_block<LPR>() / LPR, FIT = LPR <= 256 ? 4 : LPR <= 512 ? 3 : 2;
+            long parts = norm_parts(g.rows);
+            if (parts > (g.rows + RPB - 1) / RPB) parts = (g.rows + RPB - 1) / RPB;
+            if (parts > (long)FIT * device_compute_units()) parts = (long)FIT * device_compute_units();
             norm_backward_kernel<T, LPR, N><<<dim3((unsigned)parts), norm_block<LPR>(), 0, s>>>(g);
             const dim3 grid((unsigned)((g.D + 63) / 64));
             if (g.weight_f32) {
