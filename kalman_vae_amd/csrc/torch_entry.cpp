@@ -344,24 +344,30 @@ Tensor linear_8bit(const Tensor& x_in, const Tensor& x_scale_in, const Tensor& w
 }
 
 // -- optimiser --------------------------------------------------------------------------------
-// The tensors of a Python list or tuple, borrowed from it (it holds them for the call).
+bool is_list(py::handle h) { return PyTuple_Check(h.ptr()) || PyList_Check(h.ptr()); }
+
+// The items of a Python list or tuple, borrowed from it (it holds them for the call; nothing between reading
+// them and the launch runs Python code that could change it).
+c10::ArrayRef<PyObject*> items_of(py::handle list) {
+    return {PySequence_Fast_ITEMS(list.ptr()), (size_t)PySequence_Fast_GET_SIZE(list.ptr())};
+}
+
 std::vector<const Tensor*> list_of(py::handle list, const char* name) {
-    TORCH_CHECK_TYPE(PyList_Check(list.ptr()) || PyTuple_Check(list.ptr()), name, ": a list of tensors is expected");
-    const auto seq = py::reinterpret_borrow<py::sequence>(list);
+    TORCH_CHECK_TYPE(is_list(list), name, ": a list of tensors is expected");
+    const auto items = items_of(list);
     std::vector<const Tensor*> out;
-    out.reserve(seq.size());
-    for (const py::handle item : seq) {
-        TORCH_CHECK_TYPE(THPVariable_Check(item.ptr()), name, ": a list of tensors is expected");
-        out.push_back(&THPVariable_Unpack(item.ptr()));
+    out.reserve(items.size());
+    for (PyObject* item : items) {
+        TORCH_CHECK_TYPE(THPVariable_Check(item), name, ": a list of tensors is expected");
+        out.push_back(&THPVariable_Unpack(item));
     }
     return out;
 }
 
-bool is_pair(py::handle h) { return PyTuple_Check(h.ptr()) || PyList_Check(h.ptr()); }
-
 void check_list(const char* name, const std::vector<const Tensor*>& list, const std::vector<const Tensor*>& params,
                 at::ScalarType type, bool scales = false) {
     TORCH_CHECK_VALUE(list.size() == params.size(), list.size(), " ", name, " for ", params.size(), " parameters");
+    const at::Device device = params[0]->device();
     for (size_t i = 0; i < list.size(); ++i) {
         const Tensor &t = *list[i], &p = *params[i];
         TORCH_CHECK_TYPE(t.scalar_type() == type, name, ": expected ", type, ", got ", t.scalar_type());
@@ -369,26 +375,47 @@ void check_list(const char* name, const std::vector<const Tensor*>& list, const 
         TORCH_CHECK_VALUE(t.numel() == want, name, ": ", want, scales ? " scales" : " elements",
                           " expected for a parameter of ", p.numel(), " elements, got ", t.numel());
         TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
-        TORCH_CHECK_VALUE(t.device() == p.device() && t.device() == params[0]->device(), name, " on ", t.device(),
-                          ", the first parameter on ", params[0]->device());
+        TORCH_CHECK_VALUE(t.device() == device, name, " on ", t.device(), ", the first parameter on ", device);
     }
 }
 
-// Tensors that are written may not share memory: not the same one twice, not two views that overlap.
+// Tensors that are written may not share memory: not the same one twice, not two views that overlap.  Tensors
+// of different memory blocks cannot, and views of one usually come in the order of their places, so one pass
+// with the end of what has been seen of each block settles it; otherwise all are sorted.
 void check_apart(std::initializer_list<const std::vector<const Tensor*>*> lists) {
     struct Range {
         const char *begin, *end;
         bool operator<(const Range& o) const { return begin < o.begin; }
     };
+    size_t count = 0, slots = 64;
+    for (const auto* list : lists) count += list->size();
+    while (slots < 2 * count) slots *= 2;
+    struct Block {
+        const void* base;
+        const char* end;
+    };
+    std::vector<Block> seen(slots, Block{nullptr, nullptr});
+    const auto range_of = [](const Tensor& t) {
+        const char* at = static_cast<const char*>(t.data_ptr());
+        return Range{at, at + t.nbytes()};
+    };
+    bool ordered = true;
+    for (const auto* list : lists)
+        for (const Tensor* t : *list) {
+            const Range r = range_of(*t);
+            if (r.begin == r.end) continue;
+            const void* base = t->storage().data();
+            size_t at = (reinterpret_cast<uintptr_t>(base) >> 9) * 0x9E3779B97F4A7C15ull >> 32 & (slots - 1);
+            while (seen[at].base && seen[at].base != base) at = (at + 1) & (slots - 1);
+            if (seen[at].base && r.begin < seen[at].end) ordered = false;
+            seen[at] = {base, r.end};
+        }
+    if (ordered) return;
     std::vector<Range> ranges;
-    for (const auto* list : lists) {
-        ranges.reserve(ranges.size() + list->size());
+    ranges.reserve(count);
+    for (const auto* list : lists)
         for (const Tensor* t : *list)
-            if (t->numel()) {
-                const char* at = static_cast<const char*>(t->data_ptr());
-                ranges.push_back({at, at + t->nbytes()});
-            }
-    }
+            if (t->numel()) ranges.push_back(range_of(*t));
     std::sort(ranges.begin(), ranges.end());
     for (size_t i = 1; i < ranges.size(); ++i)
         TORCH_CHECK_VALUE(ranges[i].begin >= ranges[i - 1].end,
@@ -408,20 +435,23 @@ void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::
     const auto grads = list_of(grads_in, "gradients");
     check_list("gradients", grads, params, type);
     bool pairs = false, plain = false;
-    for (const auto& list : {m_in, v_in}) {
-        TORCH_CHECK_TYPE(is_pair(list), "states: lists are expected");
-        for (const py::handle item : py::reinterpret_borrow<py::sequence>(list)) (is_pair(item) ? pairs : plain) = true;
+    for (const py::handle list : {py::handle(m_in), py::handle(v_in)}) {
+        TORCH_CHECK_TYPE(is_list(list), "states: lists are expected");
+        for (PyObject* item : items_of(list)) (is_list(item) ? pairs : plain) = true;
     }
     TORCH_CHECK_TYPE(!(pairs && plain), "states are all float32 tensors or all (codes, scales) pairs");
     std::vector<const Tensor*> m, v, ms, vs, masters;
     if (pairs) {
         const auto split = [&](const py::object& list, const char* name, std::vector<const Tensor*>& codes,
                                std::vector<const Tensor*>& scales) {
-            for (const py::handle item : py::reinterpret_borrow<py::sequence>(list)) {
-                const auto two = list_of(item, name);
-                TORCH_CHECK_TYPE(two.size() == 2, name, ": (codes, scales) pairs expected");
-                codes.push_back(two[0]);
-                scales.push_back(two[1]);
+            const auto items = items_of(list);
+            codes.reserve(items.size()), scales.reserve(items.size());
+            for (PyObject* item : items) {
+                const auto two = items_of(item);
+                TORCH_CHECK_TYPE(two.size() == 2 && THPVariable_Check(two[0]) && THPVariable_Check(two[1]), name,
+                                 ": (codes, scales) pairs expected");
+                codes.push_back(&THPVariable_Unpack(two[0]));
+                scales.push_back(&THPVariable_Unpack(two[1]));
             }
             check_list(name, codes, params, at::kFloat8_e4m3fn);
             check_list(name, scales, params, at::kFloat, true);
