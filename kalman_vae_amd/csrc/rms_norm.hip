@@ -5,8 +5,8 @@
 //   dr = s (w dy - n mean(w dy n)) + g_r with n = r s,  dw = sum over rows of dy n
 //
 // Bound by memory: every input is read once and every output written once.  A row stays in the
-// registers of LPR lanes (16, 64, 256, 512 or 1024: a quarter wavefront for the narrow rows of the weight
-// network up to a whole workgroup of 16 wavefronts), N vectors of 16 bytes per lane, so that the
+// registers of LPR lanes (4, 8, 16, 64, 256, 512 or 1024: a quarter wavefront for the rows of the weight
+// network, up to a whole workgroup of 16 wavefronts), N vectors of 16 bytes per lane, so that the
 // second use of a row (after its sum of squares is known) costs no second read.
 //
 // Sums are taken in float over a lane's elements, then over the lanes by DPP exchanges and, for rows
@@ -45,10 +45,10 @@ struct Max {   // of magnitudes; a NaN is passed over
 // call site (a row wider than a wavefront only).
 template <typename OP, int LPR>
 __device__ __forceinline__ float over_row(float v, float* slot) {
-    v = OP::of(v, row_exchange<0xB1>(v));
+    v = OP::of(v, row_exchange<0xB1>(v));            // neighbours, pairs, halves of a row of 16, its mirror
     v = OP::of(v, row_exchange<0x4E>(v));
-    v = OP::of(v, row_exchange<0x141>(v));
-    v = OP::of(v, row_exchange<0x140>(v));
+    if constexpr (LPR > 4) v = OP::of(v, row_exchange<0x141>(v));
+    if constexpr (LPR > 8) v = OP::of(v, row_exchange<0x140>(v));
     if constexpr (LPR > 16)
         v = OP::of(OP::of(lane_value(v, 0), lane_value(v, 16)),
                    OP::of(lane_value(v, 32), lane_value(v, 48)));
@@ -325,24 +325,21 @@ __global__ void __launch_bounds__(norm_block<LPR>()) norm_backward_kernel(NormAr
             row_store<T, V>(static_cast<T*>(g.dx) + row * g.D, at, g.D, out);
         }
     }
-    // the workgroup's rows of lanes are added in LDS, one row of lanes after the other
+    // a wavefront's rows of lanes are added by exchanges, then the wavefronts in LDS, always in the same order
     if constexpr (RPB > 1) {
-        __shared__ float total[LPR * N * V];
-        for (int k = 0; k < RPB; ++k) {
-            __syncthreads();
-            if ((int)threadIdx.x / LPR == k) {
+        __shared__ float total[4][LPR * N * V];
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        float& t = total[(i * LPR + lane) * V + v];
-                        t = k == 0 ? dw[i][v] : t + dw[i][v];
-                    }
+            for (int v = 0; v < V; ++v) {
+                float t = dw[i][v];
+#pragma unroll
+                for (int apart = LPR; apart < 64; apart *= 2) t += __shfl_xor(t, apart);
+                if ((threadIdx.x & 63) < LPR) total[threadIdx.x >> 6][(i * LPR + lane) * V + v] = t;
             }
-        }
         __syncthreads();
         for (int at = threadIdx.x; at < g.D; at += norm_block<LPR>())
-            g.partial[(long)blockIdx.x * g.D + at] = total[at];
+            g.partial[(long)blockIdx.x * g.D + at] = total[0][at] + total[1][at] + total[2][at] + total[3][at];
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -377,7 +374,8 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(long parts, int 
 // 1024 lanes more), so that a narrow row does not leave lanes idle and the backward kernel's four rows of
 // floats leave room for four to six wavefronts to a SIMD.  (Up to four vectors of eight 16-bit elements took
 // 221 registers; backward, bfloat16: 16384 x 2048 101 us against 71, 4096 x 8192 102 against 68, 65536 x 512
-// 105 against 69; forward 45 to 51 against 43 to 45.)
+// 105 against 69; forward 45 to 51 against 43 to 45.  2500000 x 16 with 16 lanes to a row 249 us forward and
+// 425 backward, with four 79 and 132.)
 template <typename T, typename F>
 static int with_shape(int D, F&& f) {
     constexpr int V = 16 / sizeof(T);
@@ -386,6 +384,8 @@ static int with_shape(int D, F&& f) {
 #define KVAE_NORM_SHAPE(LPR, N)                                                                   \
     if (vecs <= LPR * N)                                                                          \
         return call(std::integral_constant<int, LPR>{}, std::integral_constant<int, N>{});
+    KVAE_NORM_SHAPE(4, 1)
+    KVAE_NORM_SHAPE(8, 1)
     KVAE_NORM_SHAPE(16, 1)
     KVAE_NORM_SHAPE(16, 2)
     KVAE_NORM_SHAPE(64, 1)

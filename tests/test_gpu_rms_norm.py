@@ -97,6 +97,24 @@ def test_many_rows(rows):
     check(dw, terms.sum(0), (roundings(D) + min(rows, 64 + rows // 16) * UNIT) * terms.abs().sum(0), "dw")
 
 
+@pytest.mark.parametrize("rows", [1, 63, 64, 65, 1000, 70001])
+@pytest.mark.parametrize("D", [3, 16, 17, 20, 40, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_narrow_rows(rows, D, dtype):
+    """Several rows in a quarter wavefront: outputs, and the weight gradient's sum over them."""
+    x, residual, w, dy, dsum = make(rows, D, dtype, torch.float32)
+    y, total, dx, dw, dres = run(x, residual, w, dy, dsum)
+    r, s, want = oracle(x, residual, w)
+    k = roundings(D)
+    check(y, want, k * want.abs(), "y")
+    n, d = r * s, dy.double() * w.double()
+    along, size = (d * n).mean(1, keepdim=True), (d * n).abs().mean(1, keepdim=True)
+    grad = s * (d - n * along) + dsum.double()
+    check(dx, grad, k * s * (d.abs() + 2 * n.abs() * size) + UNIT * grad.abs(), "dx")
+    terms = dy.double() * n
+    check(dw, terms.sum(0), (k + min(rows, 64 + rows // 16) * UNIT) * terms.abs().sum(0), "dw")
+
+
 def test_directional_derivative():
     x, residual, w, dy, dsum = make(9, 50, torch.float32, torch.float32)
     _, _, dx, dw, dres = run(x, residual, w, dy, dsum)
