@@ -605,11 +605,14 @@ scan_step_kernel(long B, long H, const T* __restrict__ u, long u_b, const uint8_
 // - Fewer: four wavefronts share the time axis, as long as there is more than one chunk.  At 256
 //   wavefronts and T = 1000: 57/90 against 135/210 alone; T = 20, 64 wavefronts: 4.4/6.8 against
 //   8.2/7.4.  (Eight: 5.1/8.7 there, and no faster on long sequences.)
-// - Fewer than 2048 with that: the sequence is cut into segments as well, up to 128, of at least two
-//   rounds of a workgroup each: 32768 steps of 520 half channels take 17 us to compose and 26 to
-//   run (one wavefront per segment and a launch for the start states: 47 + 10 + 54).  u is read
-//   twice then.  (Asking for the next round's steps before a round is worked on: 21 + 30, and 1000
-//   masked steps 128 -> 235, as the barrier waits for what has been asked for.)
+// - Fewer than 600 (float; 850 of a 16-bit type, whose wavefronts have half the bytes under way) with that,
+//   and six rounds of a workgroup or more: the sequence is cut into segments as well, up to 128, of at
+//   least two rounds each, and u is read twice.  T = 2000, forward and backward: float, 480 wavefronts 196
+//   against 235 uncut, 800 340 against 258; bfloat16, 600 250 against 342, 1000 460 against 382.  Float,
+//   T = 300, 480 wavefronts: 41 against 34.  32768 steps of 520 half channels take 17 us to compose and 26 to
+//   run (one wavefront per segment and a launch for the start states: 47 + 10 + 54).
+// Asking for the next round's steps before a round is worked on was slower (21 + 30 there, 1000 masked steps
+// 235 against 128): the barrier waits for what has been asked for.
 struct Plan {
     int V, L, W, segs;
     long seg;                                        // steps per segment
@@ -623,7 +626,7 @@ static Plan scan_plan(long T, long B, long H, int dtype) {
     p.segs = 1;
     p.seg = T;
     const long round = (long)p.L * p.W;
-    if (p.W > 1 && waves * p.W < 2048 && T >= 4 * round) {
+    if (p.W > 1 && waves * p.W < (dtype == KVAE_F32 ? 600 : 850) && T >= 6 * round) {
         long want = (8192 + waves * p.W - 1) / (waves * p.W);
         if (want > MOST_SEGMENTS) want = MOST_SEGMENTS;
         if (want > T / (2 * round)) want = T / (2 * round);
