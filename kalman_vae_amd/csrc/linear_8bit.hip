@@ -14,14 +14,15 @@
 // as one wide store, and the matrix instruction's k order does not matter as both sides share it.
 //
 // Three forms.  Few rows: reading w once is the work; a workgroup takes 16 rows of w (64 when there are enough
-// of them) and up to 64 of x, its wavefronts share out k and add up through LDS.  Tiles of 128 x 128 staged through registers and LDS, the
-// next slice of k on its way while the present one is multiplied, three workgroups to a unit.  Large tiles of
-// 256 x 256, fed from memory straight into LDS, for large products.
+// of them) and up to 64 of x, its wavefronts share out k and add up through LDS.  Tiles of 128 x 128 staged
+// through registers and LDS, the next slice of k on its way while the present one is multiplied, three
+// workgroups to a unit.  Large tiles of 256 x 256, fed from memory straight into LDS, for large products.
 //
-// Measured (bfloat16 results): 1 x 6144 x 2048 4.3 us (2.9 TB/s), 64 x 4096 x 4096 7 us, 1024^3 6.1, 256 x 4096 x 4096 12, 262144 x 384 x 128
-// 48 us (4.9 TB/s, memory's rate), 4096^3 58 us, 16384 x 4096 x 4096 230 us = 2.4 PFLOP/s, where the library's
-// product of 8-bit operands takes 224 us, and 8192^3 430 us = 2.6.  A loop of nothing but these instructions
-// reaches 3.4 to 4 on random bytes (the clock comes down).  Each round of large tiles spends some 12 us
+// Measured (bfloat16 results): 1 x 6144 x 2048 3.8 to 4.3 us (3 TB/s), 64 x 4096 x 4096 7 us, 256 x 4096 x 4096
+// 12 us, 1024^3 6.1 us, 262144 x 384 x 128 48 us (4.9 TB/s, memory's rate), 4096^3 58 us, 16384 x 4096 x 4096
+// 220 to 230 us = 2.4 to 2.5 PFLOP/s, where the library's product of 8-bit operands takes 224 us, and 8192^3
+// 430 us = 2.6.  A loop of nothing but these instructions reaches 3.4 to 4 on random bytes (the clock comes
+// down).  Float results: 16384 x 4096 x 4096 480 us, 262144 x 384 x 128 91 us.  Each round of large tiles spends some 12 us
 // outside its loop (first requests, results); workgroups that stay and ask for the next tile's start before
 // they write the last one's results were no faster (227 to 248 us).
 #include "narrow_types.h"

@@ -37,7 +37,7 @@ __device__ __forceinline__ float lane_value(float x, int lane) {
 struct Add {
     __device__ static float of(float a, float b) { return a + b; }
 };
-struct Max {   // of magnitudes; a NaN is passed over
+struct Max {   // a NaN is passed over
     __device__ static float of(float a, float b) { return fmaxf(a, b); }
 };
 
@@ -136,6 +136,8 @@ struct Factor {
 // (p + rest) k, rounded once: where a quotient lies next to the middle of two codes, the roundings of a
 // chain of float products would decide between them.
 __device__ __forceinline__ float times(float p, float rest, Factor k) {
+#pragma clang fp contract(off)
+    // (contracted, the last sum would hold what t leaves of the product twice)
     const float t = p * k.hi;
     return t + (__builtin_fmaf(p, k.hi, -t) + __builtin_fmaf(p, k.lo, rest * k.hi));
 }
@@ -171,7 +173,7 @@ template <typename T, int LPR, int N, bool QUANT, bool NORM>
 __global__ void __launch_bounds__(norm_block<LPR>()) norm_forward_kernel(NormArgs g) {
     constexpr int V = 16 / sizeof(T);
     constexpr int RPB = norm_block<LPR>() / LPR;   // rows a workgroup works on together
-    __shared__ float slots[2][16];
+    __shared__ float slots[3][16];
     const int lane = threadIdx.x % LPR;
     const long row = (long)blockIdx.x * RPB + threadIdx.x / LPR;
     if (LPR <= 64 && row >= g.rows) return;        // (LPR > 64: one row per workgroup, all there)
@@ -243,10 +245,20 @@ __global__ void __launch_bounds__(norm_block<LPR>()) norm_forward_kernel(NormArg
             for (int v = 0; v < V; ++v) big = fmaxf(big, fabsf(r[i][v]));
         big = over_row<Max, LPR>(big, slots[1]);
         const float scale = fmaxf(big * spread * (1.f / E4M3_MAX), SMALLEST_SCALE);
+        float more = 0.f;                          // the largest product is big + more
+        if constexpr (NORM) {
+            more = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (fabsf(r[i][v]) == big) more = fmaxf(more, r[i][v] < 0.f ? -rest[i][v] : rest[i][v]);
+            more = over_row<Max, LPR>(more, slots[2]);
+        }
         Factor k = {spread / SMALLEST_SCALE, 0.f};
         if (scale > SMALLEST_SCALE) {
             k.hi = E4M3_MAX / big;                 // spread / scale, in which spread cancels
-            if (big < __builtin_inff()) k.lo = __builtin_fmaf(-k.hi, big, E4M3_MAX) / big;
+            if (big < __builtin_inff()) k.lo = (__builtin_fmaf(-k.hi, big, E4M3_MAX) - k.hi * more) / big;
         }
         if (lane == 0) g.scale[row] = scale;
 #pragma unroll

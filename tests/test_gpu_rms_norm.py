@@ -208,6 +208,22 @@ def test_quantized(D, dtype):
     assert ((q2.double() >= low) & (q2.double() <= high)).all()
 
 
+@pytest.mark.parametrize("D", [24, 256, 1500])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_codes_are_those_of_the_quotient(D, dtype):
+    """y / scale = 448 r w / max |r w|: the codes are this quotient's, rounded to float and then to e4m3,
+    every one of them, as the kernel carries products to twice float's digits.  (Inputs on a grid on which
+    x + residual is exact, and r w is exact in float64.)"""
+    import kalman_vae_amd as kv
+    rows = 2_000_000 // D
+    x, residual, w, _, _ = make(rows, D, dtype, torch.float32, seed=D)
+    x, residual = ((t.float() * 32).round().div(32).to(dtype) for t in (x, residual))
+    q = kv.rms_norm_quantized(x, w, residual=residual, eps=EPS)[0]
+    p = (x.double() + residual.double()) * w.double()
+    t = p * (E4M3_MAX / p.abs().amax(1, keepdim=True))
+    assert torch.equal(q.double(), nearest_e4m3(t.float().double()))
+
+
 def test_empty():
     import kalman_vae_amd as kv
     w = torch.ones(5, device="cuda", requires_grad=True)
