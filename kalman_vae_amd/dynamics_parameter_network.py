@@ -182,8 +182,8 @@ class GatedModel(nn.Module):
     On a GPU in float32, bfloat16 or float16 the norms and scans are the package's HIP kernels; on the
     CPU and in float64 the module is plain torch.
 
-    ``eight_bit()`` lays the blocks' projection weights out in 8 bits; calls that record no gradient
-    then run the projections as ``linear_8bit`` on the norm's 8-bit output.  The reference has no
+    After ``eight_bit()`` calls that record no gradient run the blocks' projections as ``linear_8bit``
+    on the norm's 8-bit output.  The reference has no
     counterpart of this network (kvae/dynamics_parameter_network.py:18-90 has the LSTM and the MLP)."""
 
     eps = 1e-6
@@ -225,49 +225,62 @@ class GatedModel(nn.Module):
 
     # -- 8-bit serving form -----------------------------------------------------------------
     def eight_bit(self, on=True):
-        """Lay out (or, with ``on=False``, drop) the 8-bit form of the blocks' projections: 1 byte per
-        weight and one float32 scale per output.  Later calls without a gradient use it; a call
-        after the parameters have changed raises until this is called again.  Moving or converting the
-        module drops it.  Returns self."""
+        """Turn the 8-bit form of the blocks' projections on (or off) for the parameters as they are.
+        Calls without a gradient then make the codes, and one float32 scale per output, from the
+        weights that the model has when they run, so that none answers from former ones however they
+        were changed; an ``inference_stepper`` makes them once for its steps.  A change that autograd
+        records (in place, replaced or loaded parameters) ends the form: such calls raise until this
+        is called again.  Moving or converting the module turns it off.  Returns self."""
         self._eight = None
         if on:
             capi.require_gpu(self.norm)
-            with torch.no_grad():
-                self._eight = [tuple(quantize_rows(layer.weight) + (layer.bias.float(), layer.weight._version,
-                                                                    layer.bias._version)
-                                     for layer in (block.proj, block.out)) for block in self.blocks]
+            capi.sequence_dtype_code(self.norm.dtype)
+            if self.hidden_dim > capi.NORM_MAX_WIDTH:
+                raise NotImplementedError(f"up to {capi.NORM_MAX_WIDTH} channels, got {self.hidden_dim}")
+            self._eight = [[[(name, p, p._version) for name, p in layer._parameters.items()]
+                            for layer in (block.proj, block.out)] for block in self.blocks]
         return self
 
     def _apply(self, fn):
         self._eight = None                     # moved or converted parameters
         return super()._apply(fn)
 
-    def _product_8bit(self, i, which, q, scale, dtype):
-        weight, weight_scale, bias, *versions = self._eight[i][which]
-        layer = (self.blocks[i].proj, self.blocks[i].out)[which]
-        if versions != [layer.weight._version, layer.bias._version]:
-            raise RuntimeError("the parameters have changed since eight_bit(): call it again")
-        return linear_8bit(q, scale, weight, weight_scale, bias=bias, dtype=dtype)
+    def _check_unchanged(self, known):
+        """Raise where autograd's records show a change since eight_bit() noted `known`."""
+        for block, layers in zip(self.blocks, known):
+            for layer, params in zip((block.proj, block.out), layers):
+                if any(layer._parameters.get(name) is not p or p._version != version for name, p, version in params):
+                    raise RuntimeError("the parameters have changed since eight_bit(): call it again")
+
+    def _codes_8bit(self):
+        """[(weight codes, scales, bias) of proj and out] of every block, from the present parameters."""
+        self._check_unchanged(self._eight)
+        return [[(*quantize_rows(layer.weight), layer.bias.float()) for layer in (block.proj, block.out)]
+                for block in self.blocks]
 
     # -- forward ----------------------------------------------------------------------------
     def _on_kernels(self, x):
         return (self.use_hip_kernels and x.is_cuda and x.dtype in capi.SEQUENCE_DTYPES
                 and self.hidden_dim <= capi.NORM_MAX_WIDTH)
 
-    def _stack(self, x, scan):
-        """(branch, h) behind the last block; scan(i, u) runs block i's recurrence."""
+    def _use_8bit(self, x):
+        return self._eight is not None and self._on_kernels(x) and not torch.is_grad_enabled()
+
+    def _stack(self, x, scan, codes):
+        """The last norm's output; scan(i, u) runs block i's recurrence.  codes: see _codes_8bit; None
+        for the full form."""
         kernels = self._on_kernels(x)
-        eight = kernels and self._eight is not None and not torch.is_grad_enabled()
         h, branch = lstm_function.linear(x, self.embed), None
         for i, block in enumerate(self.blocks):
-            if eight:
+            if codes is not None:
+                (w_in, s_in, b_in), (w_out, s_out, b_out) = codes[i]
                 if branch is None:
                     q, scale = rms_norm_quantized(h, block.norm, eps=self.eps)
                 else:
                     q, scale, h = rms_norm_quantized(branch, block.norm, residual=h, eps=self.eps)
                 # (bfloat16 between the products: its rounding is far below that of 8 bits)
-                y = scan(i, self._product_8bit(i, 0, q, scale, torch.bfloat16))
-                branch = self._product_8bit(i, 1, *quantize_rows(y), x.dtype)
+                y = scan(i, linear_8bit(q, scale, w_in, s_in, bias=b_in, dtype=torch.bfloat16))
+                branch = linear_8bit(*quantize_rows(y), w_out, s_out, bias=b_out, dtype=x.dtype)
             else:
                 n, h = self._norm(h, branch, block.norm, kernels)
                 branch = lstm_function.linear(scan(i, lstm_function.linear(n, block.proj)), block.out)
@@ -297,7 +310,7 @@ class GatedModel(nn.Module):
             ends.append(end.detach() if fresh else end)
             return y
 
-        n = self._stack(x, scan)
+        n = self._stack(x, scan, self._codes_8bit() if self._use_8bit(x) else None)
         self._states = ends
         return lstm_function.softmax_head(n, self.linear, lead)
 
@@ -305,6 +318,7 @@ class GatedModel(nn.Module):
         """For a caller that feeds one step at a time without a gradient (the masked filter): an
         object whose ``step(x_t (B,a_dim), out (B,K))`` equals ``out.copy_(self(x_t[None])[0])`` with
         the state updated in place (``gated_scan_step``), or None when that form does not apply.
+        The parameters must not change before its last step (in the 8-bit form it holds their codes).
         Call ``finish_steps`` afterwards so that the module carries the state on."""
         if (torch.is_grad_enabled() or x.dim() != 2 or x.dtype != torch.float32 or not self._on_kernels(x)
                 or not lstm_function.head_supported(x.new_empty(1, self.hidden_dim), self.linear)):
@@ -323,6 +337,9 @@ class GatedStepper:
         self.model, B = model, x.shape[0]
         self.states = [torch.zeros(B, model.hidden_dim, device=x.device) if model._states is None
                        else model._states[i].clone() for i in range(model.num_layers)]
+        self.known, self.codes = None, None
+        if model._use_8bit(x):
+            self.known, self.codes = model._eight, model._codes_8bit()
 
     @torch.no_grad()
     def step(self, x, out):
@@ -331,7 +348,9 @@ class GatedStepper:
         if not (out.is_contiguous() and out.shape == (x.shape[0], model.linear.out_features)
                 and x.dtype == out.dtype == torch.float32):
             raise ValueError("GatedStepper.step: x (B,P) and contiguous out (B,K) must be float32")
-        n = model._stack(x, lambda i, u: gated_scan_step(u, self.states[i]))
+        if self.known is not None:
+            model._check_unchanged(self.known)
+        n = model._stack(x, lambda i, u: gated_scan_step(u, self.states[i]), self.codes)
         W, b = model.linear.weight.contiguous(), model.linear.bias.contiguous()
         capi.check(capi.load().kvae_softmax_head_forward(
             n.shape[0], model.hidden_dim, W.shape[0], n.data_ptr(), W.data_ptr(), b.data_ptr(),
