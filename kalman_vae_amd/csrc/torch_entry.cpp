@@ -109,6 +109,15 @@ void changed(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// A tangent of torch.autograd.forward_ad would be lost on the way through a kernel, gradient mode or not.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+template <typename... T>
+void refuse_tangents(const char* name, const T&... tensors) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(tensors) || ...) || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+                                name, " has no forward-mode derivative");
+}
+
 // Gradients of a gradient are refused when they are asked for, not when the graph is built: the first
 // ones lead to what they were made from (so that no request passes them by) through a node that raises.
 struct DifferentiableOnce : public torch::autograd::Node {
@@ -186,6 +195,7 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &u = saved[0], &mask = saved[1], &states = saved[2];
+        refuse_tangents("gated_scan's backward pass", grads[0], grads[1]);
         variable_list out(4);
         {
             at::AutoGradMode off(false);
@@ -207,6 +217,7 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
 };
 
 std::pair<Tensor, Tensor> gated_scan(const Tensor& u, const OptTensor& h0, const OptTensor& mask, bool gated) {
+    refuse_tangents("gated_scan", u, h0);
     if (at::GradMode::is_enabled() && (u.requires_grad() || (h0 && h0->requires_grad()))) {
         auto out = GatedScan::apply(rows_dense(u), h0 ? OptTensor(h0->contiguous()) : h0, mask, gated);
         return {out[0], out[1]};
@@ -216,6 +227,7 @@ std::pair<Tensor, Tensor> gated_scan(const Tensor& u, const OptTensor& h0, const
 }
 
 Tensor gated_scan_step(const Tensor& u_in, const Tensor& state, const OptTensor& mask, bool gated) {
+    refuse_tangents("gated_scan_step", u_in, state);
     const Tensor u = rows_dense(u_in);
     const On on(u);
     const int64_t B = u.size(0), H = u.size(1) / (gated ? 3 : 2);
@@ -267,6 +279,7 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &rstd = saved[3];
         variable_list out(4);
+        for (const Tensor& g : grads) refuse_tangents("rms_norm's backward pass", g);
         {
             at::AutoGradMode off(false);
             const On on(x);
@@ -292,6 +305,7 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
 
 std::pair<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight_in, const OptTensor& residual,
                                       double eps) {
+    refuse_tangents("rms_norm", x, weight_in, residual);
     const Tensor weight = weight_in.contiguous();
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || weight.requires_grad() || (residual && residual->requires_grad()))) {
@@ -304,6 +318,7 @@ std::pair<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight_in, 
 
 std::tuple<Tensor, Tensor, OptTensor> rms_norm_quantized(const Tensor& x, const Tensor& weight_in,
                                                          const OptTensor& residual, double eps) {
+    refuse_tangents("rms_norm_quantized", x, weight_in, residual);
     const On on(x);
     const int64_t D = x.size(-1);
     const Tensor weight = weight_in.contiguous();
@@ -319,6 +334,7 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_quantized(const Tensor& x, const 
 }
 
 std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
+    refuse_tangents("quantize_rows", x);
     const On on(x);
     const int64_t D = x.size(-1);
     const Rows rows(x, D);
@@ -331,6 +347,7 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
 
 Tensor linear_8bit(const Tensor& x_in, const Tensor& x_scale_in, const Tensor& w_in, const Tensor& w_scale_in,
                    const OptTensor& bias_in, at::ScalarType dtype) {
+    refuse_tangents("linear_8bit", x_scale_in, w_scale_in, bias_in);
     const On on(x_in);
     const Tensor x = x_in.contiguous(), xs = x_scale_in.contiguous(), w = w_in.contiguous(),
                  ws = w_scale_in.contiguous();
@@ -434,6 +451,7 @@ void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::
     check_list("parameters", params, params, type);
     const auto grads = list_of(grads_in, "gradients");
     check_list("gradients", grads, params, type);
+    for (size_t i = 0; i < params.size(); ++i) refuse_tangents("adamw_step", *params[i], *grads[i]);
     bool pairs = false, plain = false;
     for (const py::handle list : {py::handle(m_in), py::handle(v_in)}) {
         TORCH_CHECK_TYPE(is_list(list), "states: lists are expected");

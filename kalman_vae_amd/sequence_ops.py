@@ -4,7 +4,8 @@ root-mean-square norm with the residual's addition and its 8-bit output (csrc/rm
 the product of 8-bit rows (csrc/linear_8bit.hip).
 
 They take GPU tensors of float32, bfloat16 or float16 and run on the current stream of the
-tensors' device; states, norms and sums are float32 whatever the element type.  The
+tensors' device; states, norms and sums are float32 whatever the element type.  None has a forward-mode
+derivative: tensors with a tangent (torch.autograd.forward_ad) are refused.  The
 reference's only recurrent network is torch.nn.LSTM (kvae/dynamics_parameter_network.py:18-58);
 these operators have no counterpart there.
 """
