@@ -119,16 +119,19 @@ void refuse_tangents(const char* name, const T&... tensors) {
 }
 
 // Gradients of a gradient are refused when they are asked for, not when the graph is built: the first
-// ones lead to what they were made from (so that no request passes them by) through a node that raises.
+// ones lead through a node that raises to what they were made from, which is all that the operator's own node
+// leads to and the incoming gradients, so that no request passes them by.
 struct DifferentiableOnce : public torch::autograd::Node {
     variable_list apply(variable_list&&) override {
         TORCH_CHECK(false, "trying to differentiate twice a function that is differentiable once");
     }
 };
-variable_list once_differentiable(variable_list grads, const variable_list& made_from) {
+variable_list once_differentiable(variable_list grads, const variable_list& incoming) {
     if (!at::GradMode::is_enabled()) return grads;
     const auto node = std::make_shared<DifferentiableOnce>();
-    node->set_next_edges(torch::autograd::collect_next_edges(made_from));
+    auto edges = torch::autograd::collect_next_edges(incoming);
+    for (const auto& edge : torch::autograd::get_current_node()->next_edges()) edges.push_back(edge);
+    node->set_next_edges(std::move(edges));
     for (auto& g : grads) {
         if (!g.defined()) continue;
         g = g.detach();
@@ -212,7 +215,7 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
             with_strides(d, u, mask, dy,
                          [&] { return lib.scan_backward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream); });
         }
-        return once_differentiable(std::move(out), {u, grads[0], grads[1]});
+        return once_differentiable(std::move(out), grads);
     }
 };
 
@@ -298,7 +301,6 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
             check(lib.norm_backward(&d, on.stream));
             if (two) out[2] = out[0];
         }
-        grads.insert(grads.end(), {x, residual, weight});
         return once_differentiable(std::move(out), grads);
     }
 };
