@@ -399,8 +399,9 @@ void check_list(const char* name, const std::vector<const Tensor*>& list, const 
 }
 
 // Tensors that are written may not share memory: not the same one twice, not two views that overlap.  Tensors
-// of different memory blocks cannot, and views of one usually come in the order of their places, so one pass
-// with the end of what has been seen of each block settles it; otherwise all are sorted.
+// of different blocks of torch's allocator cannot, and views of one usually come in the order of their places, so
+// one pass with the end of what has been seen of each block settles it; otherwise, and where a storage is somebody
+// else's memory (of which there may be others, starting elsewhere), all are sorted.
 void check_apart(std::initializer_list<const std::vector<const Tensor*>*> lists) {
     struct Range {
         const char *begin, *end;
@@ -419,10 +420,12 @@ void check_apart(std::initializer_list<const std::vector<const Tensor*>*> lists)
         return Range{at, at + t.nbytes()};
     };
     bool ordered = true;
+    const c10::DeleterFnPtr torchs = c10::GetAllocator((*lists.begin())->front()->device().type())->raw_deleter();
     for (const auto* list : lists)
         for (const Tensor* t : *list) {
             const Range r = range_of(*t);
             if (r.begin == r.end) continue;
+            if (t->storage().data_ptr().get_deleter() != torchs) ordered = false;
             const void* base = t->storage().data();
             size_t at = (reinterpret_cast<uintptr_t>(base) >> 9) * 0x9E3779B97F4A7C15ull >> 32 & (slots - 1);
             while (seen[at].base && seen[at].base != base) at = (at + 1) & (slots - 1);
