@@ -791,7 +791,8 @@ int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void *x, const void 
  *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * dtype: KVAE_F32, KVAE_BF16 or KVAE_F16 of param and grad.  master: a float copy of a 16-bit
  * parameter that is updated in its place (param receives it rounded), in all tensors of a call or
- * in none.  All tensors contiguous, at any element-aligned address.
+ * in none; with follow_param an element whose param is not its master rounded (somebody has written
+ * it since) starts from param.  All tensors contiguous, at any element-aligned address.
  * state_bits 32: exp_avg, exp_avg_sq hold m and v in float.  state_bits 8: e4m3 bytes of m and of
  * sqrt(v), with a float scale per KVAE_ADAMW_BLOCK elements (the last block may be short); rounded
  * up or down by a hash of (seed, t, first_block * KVAE_ADAMW_BLOCK + element), first_block counting
@@ -816,6 +817,7 @@ typedef struct {
     int64_t step, first_block;
     double lr, beta1, beta2, eps, weight_decay;
     const void *step_device, *lr_device;
+    int32_t follow_param, _pad;
 } kvae_adamw;
 
 int kvae_adamw_step(const kvae_adamw *d, void *stream);

@@ -94,7 +94,7 @@ AdamW = _ptr_struct("AdamW", [
     "tensors", ("count", C.c_int32), ("dtype", C.c_int32), ("state_bits", C.c_int32),
     ("seed", C.c_uint32), ("step", _i64), ("first_block", _i64), ("lr", C.c_double),
     ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
-    "step_device", "lr_device"])
+    "step_device", "lr_device", ("follow_param", C.c_int32), ("_pad", C.c_int32)])
 ROLLOUT_ALL, ROLLOUT_EMIT, ROLLOUT_ADVANCE = 0, 1, 2
 
 EXPORTS = (

@@ -45,6 +45,7 @@ struct AdamArgs {
     const int64_t* step;
     const float* lr_device;
     unsigned seed;
+    int follow;
 };
 
 template <int CTRL>
@@ -208,6 +209,12 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const AdamArgs g) {
         float p[PER_LANE], grad[PER_LANE], m[PER_LANE], v[PER_LANE];
         if constexpr (MASTER) {
             load16<FULL>(static_cast<const float*>(t.master) + at, n, p);
+            if (g.follow) {                          // (2 bytes an element of 28 more to read)
+                float q[PER_LANE];
+                load16<FULL>(static_cast<const T*>(t.param) + at, n, q);
+#pragma unroll
+                for (int i = 0; i < PER_LANE; ++i) p[i] = widen(narrow<T>(p[i])) == q[i] ? p[i] : q[i];
+            }
         } else {
             load16<FULL>(static_cast<const T*>(t.param) + at, n, p);
         }
@@ -293,6 +300,7 @@ extern "C" int kvae_adamw_step(const kvae_adamw* d, void* stream) {
     g.step = static_cast<const int64_t*>(d->step_device);
     g.lr_device = static_cast<const float*>(d->lr_device);
     g.seed = d->seed;
+    g.follow = d->follow_param;
     if (!g.step) {
         g.rate = (float)(d->lr / (1.0 - pow(d->beta1, (double)d->step)));
         g.root_fix = (float)(1.0 / sqrt(1.0 - pow(d->beta2, (double)d->step)));

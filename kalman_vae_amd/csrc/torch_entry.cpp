@@ -447,7 +447,7 @@ void check_apart(std::initializer_list<const std::vector<const Tensor*>*> lists)
 
 void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::object v_in, py::object step,
                 py::object lr, double beta1, double beta2, double eps, double weight_decay, py::object masters_in,
-                int64_t seed) {
+                int64_t seed, bool follow) {
     const auto params = list_of(params_in, "parameters");
     if (params.empty()) return;
     const at::ScalarType type = params[0]->scalar_type();
@@ -492,6 +492,7 @@ void adamw_step(py::object params_in, py::object grads_in, py::object m_in, py::
     const Tensor& first = *params[0];
     d.state_bits = pairs ? 8 : 32;
     d.seed = (uint32_t)seed;
+    d.follow_param = follow;
     d.beta1 = beta1, d.beta2 = beta2, d.eps = eps, d.weight_decay = weight_decay;
     const bool counted = THPVariable_Check(step.ptr());
     if (counted) {

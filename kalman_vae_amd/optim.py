@@ -36,15 +36,17 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     holds it (then the call can be captured into a graph and replayed), in which case ``lr`` may be a
     float32 tensor of one element too.  Arithmetic is float32; nothing is allocated."""
     capi.torch_entry().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, *betas, eps, weight_decay,
-                                  masters, int(seed) & 0xFFFFFFFF)
+                                  masters, int(seed) & 0xFFFFFFFF, False)
 
 
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW``'s update through ``adamw_step``: ``state_bits=32`` (float32 states) or 8
     (2 bytes per element instead of 8).
 
-    16-bit parameters keep a float32 copy in the state that takes the updates.  Gradients have the
-    parameter's type; parameters are float32, bfloat16 or float16, contiguous and on a GPU.
+    16-bit parameters keep a float32 copy in the state that takes the updates; an element of the
+    parameter that was changed from outside (weights loaded, clipped or set between steps, by
+    whatever means) is taken over into it.  Gradients have the parameter's type; parameters are
+    float32, bfloat16 or float16, contiguous and on a GPU.
     ``capturable=True`` keeps the step count of each group on the device, so that ``step()`` can be
     captured into a HIP graph and replayed; ``lr`` may then be a float32 tensor that the caller
     changes between replays, and every parameter of the group must have a gradient from the first
@@ -121,13 +123,13 @@ class AdamW(torch.optim.Optimizer):
             for (device, dtype, step), entries in lists.items():
                 pair = lambda name: ([(s[name], s[name + "_scale"]) for _, s in entries]  # noqa: E731
                                      if group["state_bits"] == 8 else [s[name] for _, s in entries])
-                adamw_step([p for p, _ in entries],
-                           [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in entries],
-                           pair("exp_avg"), pair("exp_avg_sq"),
-                           group["step"] if group["capturable"] else step, lr=group["lr"],
-                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                           masters=[s["master"] for _, s in entries] if dtype != torch.float32 else None,
-                           seed=group["seed"] + 0x51ED2701 * salt)
+                capi.torch_entry().adamw_step(
+                    [p for p, _ in entries],
+                    [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in entries],
+                    pair("exp_avg"), pair("exp_avg_sq"), group["step"] if group["capturable"] else step, group["lr"],
+                    *group["betas"], group["eps"], group["weight_decay"],
+                    [s["master"] for _, s in entries] if dtype != torch.float32 else None,
+                    (int(group["seed"]) + 0x51ED2701 * salt) & 0xFFFFFFFF, True)
                 salt += 1
         return loss
 
