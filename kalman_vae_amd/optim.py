@@ -48,7 +48,8 @@ class AdamW(torch.optim.Optimizer):
     whatever means) is taken over into it.  Gradients have the parameter's type; parameters are
     float32, bfloat16 or float16, contiguous and on a GPU.
     ``capturable=True`` keeps the step count of each group on the device, so that ``step()`` can be
-    captured into a HIP graph and replayed; ``lr`` may then be a float32 tensor that the caller
+    captured into a HIP graph and replayed (the first step, which makes the states, outside the
+    capture; a loaded state dict needs a new one); ``lr`` may then be a float32 tensor that the caller
     changes between replays, and every parameter of the group must have a gradient from the first
     step on, or never."""
 
@@ -105,6 +106,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._check_capture()
         salt = 0                        # lists of one step draw different random bits
         for group in self.param_groups:
             lists = {}
@@ -132,6 +134,19 @@ class AdamW(torch.optim.Optimizer):
                     (int(group["seed"]) + 0x51ED2701 * salt) & 0xFFFFFFFF, True)
                 salt += 1
         return loss
+
+    def _check_capture(self):
+        """A replay repeats what was captured: a count that the host passes would stand still, states that
+        are made inside the capture would be cleared each time."""
+        if not (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
+            return
+        for group in self.param_groups:
+            given = [p for p in group["params"] if p.grad is not None]
+            if given and not group["capturable"]:
+                raise RuntimeError("AdamW.step() is being captured into a graph: this needs capturable=True")
+            if not all(self.state.get(p) for p in given):
+                raise RuntimeError("AdamW.step() is being captured into a graph, but a parameter has no state yet: "
+                                   "run a step before the capture")
 
     def _device_step(self, group, lists):
         """Advance the group's step count on the device (one launch, captured with the step)."""
