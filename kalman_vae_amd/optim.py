@@ -118,20 +118,26 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p, group))
-                state["step"] += 1
-                lists.setdefault((p.device, p.dtype, state["step"]), []).append((p, state))
-            if group["capturable"]:
+                lists.setdefault((p.device, p.dtype, state["step"] + 1), []).append((p, state))
+            if group["capturable"] and lists:
                 self._device_step(group, lists)
-            for (device, dtype, step), entries in lists.items():
+            for n, ((device, dtype, step), entries) in enumerate(lists.items()):
                 pair = lambda name: ([(s[name], s[name + "_scale"]) for _, s in entries]  # noqa: E731
                                      if group["state_bits"] == 8 else [s[name] for _, s in entries])
-                capi.torch_entry().adamw_step(
-                    [p for p, _ in entries],
-                    [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in entries],
-                    pair("exp_avg"), pair("exp_avg_sq"), group["step"] if group["capturable"] else step, group["lr"],
-                    *group["betas"], group["eps"], group["weight_decay"],
-                    [s["master"] for _, s in entries] if dtype != torch.float32 else None,
-                    (int(group["seed"]) + 0x51ED2701 * salt) & 0xFFFFFFFF, True)
+                try:
+                    capi.torch_entry().adamw_step(
+                        [p for p, _ in entries],
+                        [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in entries],
+                        pair("exp_avg"), pair("exp_avg_sq"), group["step"] if group["capturable"] else step,
+                        group["lr"], *group["betas"], group["eps"], group["weight_decay"],
+                        [s["master"] for _, s in entries] if dtype != torch.float32 else None,
+                        (int(group["seed"]) + 0x51ED2701 * salt) & 0xFFFFFFFF, True)
+                except Exception:                    # refused: no step has been made
+                    if group["capturable"] and n == 0:
+                        group["step"].sub_(1)
+                    raise
+                for _, state in entries:
+                    state["step"] = step
                 salt += 1
         return loss
 
@@ -153,8 +159,6 @@ class AdamW(torch.optim.Optimizer):
         if len({step for _, _, step in lists}) > 1 or len({device for device, _, _ in lists}) > 1:
             raise RuntimeError("capturable=True: the parameters of a group share one step count on one "
                                "device, so each needs a gradient in every step, or in none")
-        if not lists:
-            return
         if group.get("step") is None:
             device = next(iter(lists))[0]
             group["step"] = torch.zeros(1, dtype=torch.int64, device=device)
