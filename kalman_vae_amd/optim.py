@@ -88,7 +88,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch.optim.Optimizer, which would convert every floating-point state to the
-        parameter's type: the states are taken over in their own."""
+        parameter's type: the states are taken over in their own.  A step count and a rate that are
+        tensors go to the parameters' device, from wherever they were loaded."""
         super().load_state_dict(state_dict)
         params = [p for g in self.param_groups for p in g["params"]]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -97,8 +98,9 @@ class AdamW(torch.optim.Optimizer):
                 if isinstance(value, torch.Tensor):
                     self.state[p][name] = value.detach().to(p.device, copy=True)
         for g, saved in zip(self.param_groups, state_dict["param_groups"]):
-            if isinstance(saved.get("step"), torch.Tensor):
-                g["step"] = saved["step"].detach().to(g["params"][0].device, copy=True)
+            for name in ("step", "lr"):
+                if isinstance(saved.get(name), torch.Tensor):
+                    g[name] = saved[name].detach().to(g["params"][0].device, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None):
