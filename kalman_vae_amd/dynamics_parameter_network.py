@@ -241,9 +241,9 @@ class GatedModel(nn.Module):
                             for layer in (block.proj, block.out)] for block in self.blocks]
         return self
 
-    def _apply(self, fn):
+    def _apply(self, fn, recurse=True):
         self._eight = None                     # moved or converted parameters
-        return super()._apply(fn)
+        return super()._apply(fn, recurse)
 
     def _check_unchanged(self, known):
         """Raise where autograd's records show a change since eight_bit() noted `known`."""
