@@ -98,8 +98,8 @@ class StateSpaceModel(nn.Module):
         self.in_kernel_weight_network = True
         self.check_numerics = True  # raise on a non-positive-definite covariance (host sync)
 
-    def _apply(self, fn):
-        super()._apply(fn)
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
         for name in ("_a_eye", "_z_eye", "initial_state_mean", "initial_state_covariance"):
             setattr(self, name, fn(getattr(self, name)))
         return self
