@@ -796,8 +796,8 @@ int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void *x, const void 
  * state_bits 32: exp_avg, exp_avg_sq hold m and v in float.  state_bits 8: e4m3 bytes of m and of
  * sqrt(v), with a float scale per KVAE_ADAMW_BLOCK elements (the last block may be short); rounded
  * up or down by a hash of (seed, t, first_block * KVAE_ADAMW_BLOCK + element), first_block counting
- * the blocks of the tensors of earlier calls of the same step, so that no two share their bits.  A
- * positive sqrt(v) never gets the code 0.
+ * the blocks of the tensors of earlier calls of the same step, so that no two of up to 2^32 elements
+ * share their bits (those beyond draw others, as if at random).  A positive sqrt(v) never gets the code 0.
  * t = step >= 1, or *step_device (int64) when that is not NULL: then the launch may be captured and
  * replayed; lr_device (float, or NULL) likewise replaces lr.                                 */
 #define KVAE_ADAMW_BLOCK 256
