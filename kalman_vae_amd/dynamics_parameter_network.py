@@ -7,6 +7,8 @@ Linear+softmax head); on the CPU they are plain torch.  Parameter names match th
 reference (kvae/dynamics_parameter_network.py:18-90) so its checkpoints load:
 ``lstm.*`` + ``linear.*`` for the LSTM model, ``layers.<i>.*`` for the MLP.
 """
+import contextlib
+
 import torch
 import torch.nn as nn
 
@@ -140,6 +142,13 @@ class MLPModel(nn.Module):
             x = torch.relu(lstm_function.linear(x, layer))
 
     is_recurrent = False
+
+
+def _device_of(x):
+    """x's device as the current one, for what launches on the current device's stream."""
+    if not x.is_cuda or x.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(x.device)
 
 
 def _plain_norm(x, weight, eps):
@@ -310,9 +319,10 @@ class GatedModel(nn.Module):
             ends.append(end.detach() if fresh else end)
             return y
 
-        n = self._stack(x, scan, self._codes_8bit() if self._use_8bit(x) else None)
-        self._states = ends
-        return lstm_function.softmax_head(n, self.linear, lead)
+        with _device_of(x):
+            n = self._stack(x, scan, self._codes_8bit() if self._use_8bit(x) else None)
+            self._states = ends
+            return lstm_function.softmax_head(n, self.linear, lead)
 
     def inference_stepper(self, x):
         """For a caller that feeds one step at a time without a gradient (the masked filter): an
@@ -350,11 +360,12 @@ class GatedStepper:
             raise ValueError("GatedStepper.step: x (B,P) and contiguous out (B,K) must be float32")
         if self.known is not None:
             model._check_unchanged(self.known)
-        n = model._stack(x, lambda i, u: gated_scan_step(u, self.states[i]), self.codes)
-        W, b = model.linear.weight.contiguous(), model.linear.bias.contiguous()
-        capi.check(capi.load().kvae_softmax_head_forward(
-            n.shape[0], model.hidden_dim, W.shape[0], n.data_ptr(), W.data_ptr(), b.data_ptr(),
-            out.data_ptr(), 0, capi.current_stream_ptr()))
+        with _device_of(x):
+            n = model._stack(x, lambda i, u: gated_scan_step(u, self.states[i]), self.codes)
+            W, b = model.linear.weight.contiguous(), model.linear.bias.contiguous()
+            capi.check(capi.load().kvae_softmax_head_forward(
+                n.shape[0], model.hidden_dim, W.shape[0], n.data_ptr(), W.data_ptr(), b.data_ptr(),
+                out.data_ptr(), 0, capi.current_stream_ptr()))
 
 
 def make_weight_model(kind, a_dim, K, hidden_dim, num_layers):
