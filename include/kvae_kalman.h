@@ -778,7 +778,9 @@ int kvae_quantize_rows(int64_t rows, int64_t D, int dtype, const void *x, int64_
 /* Product of 8-bit rows, y (M,N) = (x w^T) * x_scale[m] * w_scale[n] + bias[n]: the projection that
  * reads kvae_rms_norm_quantized's output in the serving form of the "gated" network.  x (M,K) and
  * w (N,K) contiguous e4m3 bytes at any address, x_scale (M), w_scale (N) and bias (N, or NULL) float;
- * sums in float; y of out_dtype (KVAE_F32, KVAE_BF16 or KVAE_F16).  K up to 2^22, N up to 2^26,
+ * y of out_dtype (KVAE_F32, KVAE_BF16 or KVAE_F16), rounded once.  Sums are float for KVAE_F32 and for up
+ * to 32 rows; 16-bit results of more rows lose, of each eight neighbouring products, what lies below 2^-13
+ * of the largest (the matrix instructions for 8-bit operands).  K up to 2^22, N up to 2^26,
  * M up to 2^31, M N up to 2^40.                                                             */
 int kvae_linear_8bit(int64_t M, int64_t N, int64_t K, const void *x, const void *x_scale,
                      const void *w, const void *w_scale, const void *bias, int out_dtype, void *y,

@@ -2,12 +2,16 @@
 // e4m3 with one float scale per row (what rms_norm_quantized and quantize_rows write), summed in
 // float on the matrix instructions.
 //
-// 16-bit results take the instructions for 8-bit operands.  These add eight neighbouring products
-// aligned to the largest of them and drop what lies 2^-14 or more below it (seen by feeding them one
-// large and one small product, at every distance), 1.6e-5 of a sum of Gaussian terms: a hundredth of
-// a bfloat16 result's rounding and a fifteenth of a half's.  A float result would show it, so there
-// the bytes are widened to half, which holds every e4m3 value, and multiplied by the instructions for
-// half operands, at half the rate, whose sums are float throughout (1e-8 on the same terms).
+// 16-bit results of more than 32 rows take the instructions for 8-bit operands.  These add eight neighbouring
+// products aligned to the largest of them and drop what lies 2^-14 or more below it (seen by feeding them one
+// large and one small product, at every distance): each of the other seven loses less than 2^-13 of the largest.
+// That is 1.6e-5 of a sum of Gaussian terms, a hundredth of a bfloat16 result's rounding and a fifteenth of a
+// half's, but more than float sums lose, and all of a small result where large products cancel.  Otherwise the
+// bytes are widened to half, which holds every e4m3 value, and multiplied by the instructions for half operands,
+// at half the rate, whose sums are float throughout (1e-8 on the same terms): for float results, which would show
+// the difference, and for up to 32 rows, where reading w takes as long either way (bfloat16, 8-bit operands
+// against widened ones: 1 x 6144 x 2048 4.84 against 4.94 us, 32 x 4096 x 4096 6.82 against 6.94; 64 rows 7.9
+// against 8.8, 16384 x 4096 x 4096 230 against 480).
 //
 // Both operands lie along k, so a lane's 32 operand bytes are contiguous in memory.  w takes the
 // first operand's place: then a lane's results are four neighbouring n of one row m, which go out
@@ -80,9 +84,9 @@ __device__ __forceinline__ v8h widen8(const v8i& a, int i) {
     return v8h{p.x, p.y, q.x, q.y, r.x, r.y, t.x, t.y};
 }
 
-// whether results of this type need the products of widened operands
-template <typename T>
-constexpr bool WIDENED = sizeof(T) == 4;
+// whether results of this type, from blocks of 16 MT rows of x, take the products of widened operands
+template <typename T, int MT = 4>
+constexpr bool WIDENED = sizeof(T) == 4 || MT <= 2;
 
 // four neighbouring results of one row
 template <typename T>
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) linear_few_rows_kernel(LinearA
         v8i a[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) a[u] = operand(u);
-        if constexpr (WIDENED<T>) {
+        if constexpr (WIDENED<T, MT>) {
             // (quarter by quarter, so that the widened operands of one only are in registers)
             v8i b[MT];
 #pragma unroll

@@ -190,9 +190,13 @@ def linear_8bit(x, x_scale, weight, weight_scale, bias=None, dtype=torch.float32
     (...) as ``rms_norm_quantized`` returns them, weight (N, K) with weight_scale (N) as
     ``quantize_rows`` lays them out once; y (..., N) of ``dtype`` (float32, bfloat16 or float16).
 
-    The sum runs over the 8-bit values on the matrix instructions in float32; scales and bias
-    (float32) are applied before the one rounding to ``dtype``.  Any sizes.  Serving only: no
-    gradient."""
+    Scales and bias (float32) are applied to the sum of the products of the 8-bit values, before the one
+    rounding to ``dtype``.  The sum is float32 throughout with ``dtype=torch.float32``, and with up to 32
+    rows of x.  16-bit results of more rows come from the matrix instructions for 8-bit operands, at twice
+    the rate: of every eight neighbouring products these cut what lies below 2^-13 of the largest
+    (1e-5 of a sum of terms of like size; where larger products cancel, a small result may be lost, and
+    float32 results rounded afterwards are the way to have it).  K up to 2^22, N up to 2^26, M up to 2^31
+    rows, M N up to 2^40.  Serving only: no gradient."""
     _device_of(x, x_scale, weight, weight_scale, bias)
     capi.sequence_dtype_code(dtype)
     for name, t in (("x", x), ("weight", weight)):
