@@ -35,7 +35,7 @@ static_assert(QUANT_BLOCK == 16 * PER_LANE, "a block is one row of 16 lanes");
 struct AdamArgs {
     kvae_adamw_tensor t[TABLE];
     int first_chunk[TABLE + 1];                      // workgroup -> tensor
-    long first_block[TABLE];                         // blocks of 256 of the tensors before (hash index)
+    unsigned first_block[TABLE];                     // blocks of 256 of the tensors before (hash index)
     int count;
     float lr, beta1, beta2, eps, decay;              // decay: lr * weight_decay
     float one_minus_beta1, one_minus_beta2;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const AdamArgs g) {
         if constexpr (EIGHT) {
             const bool first = inside == 0;
             // elements 2^32 apart have the same low half of the index: the high one gives them another key
-            const unsigned long index = (unsigned long)(g.first_block[low] * QUANT_BLOCK + at);
+            const unsigned long index = (unsigned long)g.first_block[low] * QUANT_BLOCK + (unsigned long)at;
             const unsigned high = (unsigned)(index >> 32);
             if (high) key = random_bits(key + high * INDEX_FACTOR);
             const unsigned h = (unsigned)index * INDEX_FACTOR + key;
@@ -289,7 +289,7 @@ extern "C" int kvae_adamw_step(const kvae_adamw* d, void* stream) {
         if ((t.master != nullptr) != master) return KVAE_E_BADARG;
         g.t[i] = t;
         g.first_chunk[i] = (int)chunks;
-        g.first_block[i] = blocks;
+        g.first_block[i] = (unsigned)blocks;
         chunks += (t.numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
         blocks += (t.numel + QUANT_BLOCK - 1) / QUANT_BLOCK;
         if (chunks >= (1L << 32) / ADAM_THREADS) return KVAE_E_TOOLARGE;   // a launch has fewer than 2^32 threads

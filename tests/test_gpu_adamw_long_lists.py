@@ -40,7 +40,7 @@ def call(n, first_block):
     return before, [m[0], v[0]]
 
 
-@pytest.mark.parametrize("first_block", [0, 1000, (1 << 24) - 3, 1 << 24, (1 << 24) + 1000, (3 << 24) + 7, 1 << 40])
+@pytest.mark.parametrize("first_block", [0, 1000, (1 << 24) - 3, 1 << 24, (1 << 24) + 1000, (3 << 24) + 7, 1 << 31])
 def test_codes_follow_the_rule(first_block):
     n = 5000                                     # (one case begins three blocks before the border)
     (m0, r0, g), got = call(n, first_block)
