@@ -112,6 +112,12 @@ class AdamW(torch.optim.Optimizer):
         salt = 0                        # lists of one step draw different random bits
         for group in self.param_groups:
             lists = {}
+            if not group["capturable"] and group.get("step") is not None:
+                # (no longer capturable: the device's count is the one that replays have advanced)
+                count = int(group.pop("step"))
+                for p in group["params"]:
+                    if self.state.get(p):
+                        self.state[p]["step"] = count
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -162,6 +168,6 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("capturable=True: the parameters of a group share one step count on one "
                                "device, so each needs a gradient in every step, or in none")
         if group.get("step") is None:
-            device = next(iter(lists))[0]
-            group["step"] = torch.zeros(1, dtype=torch.int64, device=device)
+            device, _, step = next(iter(lists))
+            group["step"] = torch.full((1,), step - 1, dtype=torch.int64, device=device)
         group["step"].add_(1)
