@@ -22,13 +22,15 @@
 // through registers and LDS, the next slice of k on its way while the present one is multiplied, three
 // workgroups to a unit.  Large tiles of 256 x 256, fed from memory straight into LDS, for large products.
 //
-// Measured (bfloat16 results): 1 x 6144 x 2048 3.8 to 4.3 us (3 TB/s), 64 x 4096 x 4096 7 us, 256 x 4096 x 4096
-// 12 us, 1024^3 6.1 us, 262144 x 384 x 128 48 us (4.9 TB/s, memory's rate), 4096^3 58 us, 16384 x 4096 x 4096
-// 220 to 230 us = 2.4 to 2.5 PFLOP/s, where the library's product of 8-bit operands takes 224 us, and 8192^3
-// 430 us = 2.6.  A loop of nothing but these instructions reaches 3.4 to 4 on random bytes (the clock comes
-// down).  Float results: 16384 x 4096 x 4096 480 us, 262144 x 384 x 128 91 us.  Each round of large tiles spends some 12 us
-// outside its loop (first requests, results); workgroups that stay and ask for the next tile's start before
-// they write the last one's results were no faster (227 to 248 us).
+// Measured (bfloat16 results, kernel times).  The same operands call after call: 1 x 6144 x 2048 3.8 us (3.3 TB/s),
+// 64 x 4096 x 4096 7 us, 256 x 4096 x 4096 11 us, 1024^3 6.3 us, 262144 x 384 x 128 48 us (4.9 TB/s, memory's rate),
+// 4096^3 58 us, 16384 x 4096 x 4096 220 us = 2.5 PFLOP/s, 8192^3 446 us = 2.5.  Rows that were not used just before:
+// 1 x 6144 x 2048 4.2 us (weights too: 4.9), 262144 x 384 x 128 54, 16384 x 4096 x 4096 230 to 250, where the library's
+// product of 8-bit operands takes 224 us.  A loop of nothing but these instructions reaches 3.4 to 4 PFLOP/s on random
+// bytes (the clock comes down).  k = 4097 goes to tiles of 128: 495 us.  Float results, on new rows: 16384 x 4096 x
+// 4096 590 us, where the library's product of half operands takes 550; 262144 x 384 x 128 94 us, 262144 x 128 x 128 30.
+// Each round of large tiles spends some 12 us outside its loop (first requests, results); workgroups that stay and
+// ask for the next tile's start before they write the last one's results were no faster (227 to 248 us).
 #include "narrow_types.h"
 
 #include "device_info.h"

@@ -5,8 +5,10 @@ the product of 8-bit rows (csrc/linear_8bit.hip).
 
 They take GPU tensors of float32, bfloat16 or float16 and run on the current stream of the
 tensors' device; states, norms and sums are float32 whatever the element type.  None has a forward-mode
-derivative: tensors with a tangent (torch.autograd.forward_ad) are refused.  The
-reference's only recurrent network is torch.nn.LSTM (kvae/dynamics_parameter_network.py:18-58);
+derivative: tensors with a tangent (torch.autograd.forward_ad) are refused.  Only the product's
+16-bit results of more than 32 rows come from sums of fewer bits (see linear_8bit).
+
+The reference's only recurrent network is torch.nn.LSTM (kvae/dynamics_parameter_network.py:18-58);
 these operators have no counterpart there.
 """
 import torch
@@ -71,8 +73,9 @@ def gated_scan(u, h0=None, mask=None, output_gate=True):
     lie 2^31 bytes apart.  T = 0 returns ``h0`` as the last state.
 
     Differentiable (once) with respect to ``u`` and ``h0``.  The backward pass reads u and the
-    gradients and a float32 state per 16 steps that the forward pass keeps; the state and every sum
-    are float32, results are rounded to u's type once, and repeated calls give the same bits.
+    gradients and a float32 state per 16 steps (float32; 8 steps of the 16-bit types) that the
+    forward pass keeps; the state and every sum are float32, results are rounded to u's type once, and
+    repeated calls give the same bits.
     """
     _device_of(u, h0, mask)
     if u.dim() != 3:
@@ -173,7 +176,8 @@ def _empty_quantized(x):
 
 def quantize_rows(x):
     """The last axis of x in 8 bits with one scale per row: ``(q, scale)`` as in
-    ``rms_norm_quantized`` without the norm.  Lays out the weights of ``linear_8bit`` once."""
+    ``rms_norm_quantized`` without the norm.  Lays out the weights of ``linear_8bit`` once.  Rows of up to
+    16384 elements; longer ones need codes and scales of the caller's own."""
     _device_of(x)
     capi.sequence_dtype_code(x.dtype)
     if x.dim() < 1:
