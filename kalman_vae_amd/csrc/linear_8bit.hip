@@ -9,9 +9,10 @@
 // half's, but more than float sums lose, and all of a small result where large products cancel.  Otherwise the
 // bytes are widened to half, which holds every e4m3 value, and multiplied by the instructions for half operands,
 // at half the rate, whose sums are float throughout (1e-8 on the same terms): for float results, which would show
-// the difference, and for up to 32 rows, where reading w takes as long either way (bfloat16, 8-bit operands
-// against widened ones: 1 x 6144 x 2048 4.84 against 4.94 us, 32 x 4096 x 4096 6.82 against 6.94; 64 rows 7.9
-// against 8.8, 16384 x 4096 x 4096 230 against 480).
+// the difference, and for up to 32 rows, where reading w is most of the work (bfloat16, 8-bit operands against
+// widened ones, weights not used just before: 1 x 6144 x 2048 4.84 us both, 32 x 4096 x 4096 6.82 both, 64 rows 7.9
+// against 8.8; the same weights call after call: 3.85 against 4.3 and 6.0 against 6.2; 16384 x 4096 x 4096 220
+// against 475).
 //
 // Both operands lie along k, so a lane's 32 operand bytes are contiguous in memory.  w takes the
 // first operand's place: then a lane's results are four neighbouring n of one row m, which go out
@@ -22,13 +23,14 @@
 // through registers and LDS, the next slice of k on its way while the present one is multiplied, three
 // workgroups to a unit.  Large tiles of 256 x 256, fed from memory straight into LDS, for large products.
 //
-// Measured (bfloat16 results, kernel times).  The same operands call after call: 1 x 6144 x 2048 3.8 us (3.3 TB/s),
-// 64 x 4096 x 4096 7 us, 256 x 4096 x 4096 11 us, 1024^3 6.3 us, 262144 x 384 x 128 48 us (4.9 TB/s, memory's rate),
-// 4096^3 58 us, 16384 x 4096 x 4096 220 us = 2.5 PFLOP/s, 8192^3 446 us = 2.5.  Rows that were not used just before:
-// 1 x 6144 x 2048 4.2 us (weights too: 4.9), 262144 x 384 x 128 54, 16384 x 4096 x 4096 230 to 250, where the library's
+// Measured (bfloat16 results, kernel times).  The same operands call after call: 1 x 6144 x 2048 4.3 us (2.9 TB/s),
+// 64 x 4096 x 4096 7 to 8.4 us, 256 x 4096 x 4096 12 us, 1024^3 6.5 us, 262144 x 384 x 128 48 us (4.9 TB/s, memory's
+// rate), 4096^3 58 us, 16384 x 4096 x 4096 222 us = 2.5 PFLOP/s, 8192^3 432 us = 2.5.  Operands that were not used just
+// before: 1 x 6144 x 2048 4.8 us, 262144 x 384 x 128 54, 16384 x 4096 x 4096 240 to 265, where the library's
 // product of 8-bit operands takes 224 us.  A loop of nothing but these instructions reaches 3.4 to 4 PFLOP/s on random
-// bytes (the clock comes down).  k = 4097 goes to tiles of 128: 495 us.  Float results, on new rows: 16384 x 4096 x
-// 4096 590 us, where the library's product of half operands takes 550; 262144 x 384 x 128 94 us, 262144 x 128 x 128 30.
+// bytes (the clock comes down).  k = 4097 goes to tiles of 128: 450 us (495).  Float results: 16384 x 4096 x 4096
+// 475 us (on new rows 565, where the library's product of half operands takes 510 to 550), 262144 x 384 x 128 89 us,
+// 262144 x 128 x 128 29.
 // Each round of large tiles spends some 12 us outside its loop (first requests, results); workgroups that stay and
 // ask for the next tile's start before they write the last one's results were no faster (227 to 248 us).
 #include "narrow_types.h"
