@@ -125,18 +125,29 @@ void refuse_tangents(const char* name, const T&... tensors) {
 }
 
 // Gradients of a gradient are refused when they are asked for, not when the graph is built: the first
-// ones lead through a node that raises to what they were made from, which is all that the operator's own node
-// leads to and the incoming gradients, so that no request passes them by.
+// ones lead through a node that raises to what they were made from, the operator's inputs and the incoming
+// gradients, so that no request passes them by.  (The inputs' edges are noted when the operator runs: its node is
+// not known to a backward pass that is called by hand, and an input that is not read there need not be kept.)
+struct Edges : torch::CustomClassHolder {
+    explicit Edges(torch::autograd::edge_list l) : list(std::move(l)) {}
+    torch::autograd::edge_list list;
+};
+template <typename... T>
+void note_inputs(AutogradContext* ctx, const T&... inputs) {
+    ctx->saved_data["inputs"] =
+        c10::IValue::make_capsule(c10::make_intrusive<Edges>(torch::autograd::collect_next_edges(inputs...)));
+}
 struct DifferentiableOnce : public torch::autograd::Node {
     variable_list apply(variable_list&&) override {
         TORCH_CHECK(false, "trying to differentiate twice a function that is differentiable once");
     }
 };
-variable_list once_differentiable(variable_list grads, const variable_list& incoming) {
+variable_list once_differentiable(AutogradContext* ctx, variable_list grads, const variable_list& incoming) {
     if (!at::GradMode::is_enabled()) return grads;
     const auto node = std::make_shared<DifferentiableOnce>();
     auto edges = torch::autograd::collect_next_edges(incoming);
-    for (const auto& edge : torch::autograd::get_current_node()->next_edges()) edges.push_back(edge);
+    const auto inputs = ctx->saved_data["inputs"].toCapsule();
+    for (const auto& edge : static_cast<const Edges&>(*inputs).list) edges.push_back(edge);
     node->set_next_edges(std::move(edges));
     for (auto& g : grads) {
         if (!g.defined()) continue;
@@ -196,6 +207,7 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
                                  const OptTensor& mask, bool gated) {
         auto out = scan_forward(u, h0, mask, gated, true);
         ctx->save_for_backward({u, mask.value_or(Tensor()), out[2]});
+        note_inputs(ctx, u, h0.value_or(Tensor()));
         ctx->saved_data["gated"] = gated;
         ctx->saved_data["h0"] = h0.has_value();
         ctx->set_materialize_grads(false);
@@ -221,7 +233,7 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
             with_strides(d, u, mask, dy,
                          [&] { return lib.scan_backward(&d, ws.data_ptr(), (size_t)ws.numel(), on.stream); });
         }
-        return once_differentiable(std::move(out), grads);
+        return once_differentiable(ctx, std::move(out), grads);
     }
 };
 
@@ -281,6 +293,7 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
         // formed again from x and residual (one tensor more to read).
         const bool again = residual && x.scalar_type() != at::kFloat;
         ctx->save_for_backward({residual && !again ? out[1] : x, again ? *residual : Tensor(), weight, out[2]});
+        note_inputs(ctx, x, weight, residual.value_or(Tensor()));
         ctx->set_materialize_grads(false);
         return residual ? variable_list{out[0], out[1]} : variable_list{out[0]};
     }
@@ -307,7 +320,7 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
             check(lib.norm_backward(&d, on.stream));
             if (two) out[2] = out[0];
         }
-        return once_differentiable(std::move(out), grads);
+        return once_differentiable(ctx, std::move(out), grads);
     }
 };
 

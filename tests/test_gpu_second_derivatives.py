@@ -51,3 +51,20 @@ def test_start_state_may_change_before_the_backward_pass():
         leaves["h0"].add_(1.0)
     got = torch.autograd.grad((y.sum(), last.sum()), list(leaves.values()))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("square", [False, True])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_backward_pass_called_by_hand(case, square):
+    """The operator's node called outside a backward pass: the same gradients, and the same refusal."""
+    leaves, out = CASES[case]()
+    total = sum((o.square() if square else o).sum() for o in out)
+    want = torch.autograd.grad(total, list(leaves.values()), retain_graph=True)
+    incoming = torch.autograd.grad(total, out, retain_graph=True, create_graph=square)
+    got = [g for g in out[0].grad_fn(*incoming) if g is not None]
+    assert len(got) == len(want)
+    # (the norm's node has x, weight and residual in this order; between it and a leaf a conversion may stand)
+    assert all(torch.equal(g.float(), w) for g, w in zip(got, want))
+    for second in leaves.values():
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(got[0].sum(), second, retain_graph=True, allow_unused=True)
