@@ -53,6 +53,8 @@ class AdamW(torch.optim.Optimizer):
     changes between replays, and every parameter of the group must have a gradient from the first
     step on, or never."""
 
+    _former_counts = ()
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  seed=0, capturable=False):
         if not isinstance(lr, torch.Tensor) and lr < 0:
@@ -113,8 +115,10 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             lists = {}
             if not group["capturable"] and group.get("step") is not None:
-                # (no longer capturable: the device's count is the one that replays have advanced)
-                count = int(group.pop("step"))
+                # no longer capturable: the device's count is the one that replays have advanced (it is kept, as
+                # graphs that were captured write it)
+                self._former_counts += (group["step"],)
+                count, group["step"] = int(group["step"]), None
                 for p in group["params"]:
                     if self.state.get(p):
                         self.state[p]["step"] = count

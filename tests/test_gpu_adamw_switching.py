@@ -1,4 +1,6 @@
 """``capturable`` switched in the middle of a run: the step count goes on."""
+import copy
+
 import pytest
 import torch
 
@@ -68,3 +70,21 @@ def test_after_replays():
     go(ps, opt, range(5, 8))
     go(qs, plain, range(8))
     assert same(ps, qs) and all(opt.state[p]["step"] == 8 for p in ps)
+
+
+def test_counts_of_former_graphs_stay_allocated():
+    """A graph that was captured before the switch still writes its count: nothing else gets that memory."""
+    ps = parameters()
+    opt = AdamW(ps, capturable=True)
+    go(ps, opt, range(2))
+    place = opt.param_groups[0]["step"].data_ptr()
+    opt.param_groups[0]["capturable"] = False
+    go(ps, opt, range(2, 4))
+    others = [torch.empty(1, dtype=torch.int64, device="cuda") for _ in range(1000)]
+    assert place not in {t.data_ptr() for t in others}
+    opt.param_groups[0]["capturable"] = True
+    go(ps, opt, range(4, 5))
+    assert int(opt.param_groups[0]["step"]) == 5 and opt.param_groups[0]["step"].data_ptr() != place
+    again = copy.deepcopy(opt)                   # (what a copy lacks is not missed)
+    again.param_groups[0]["capturable"] = False
+    go(again.param_groups[0]["params"], again, range(5, 6))
